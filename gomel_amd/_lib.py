@@ -85,6 +85,19 @@ SYMBOLS = {
     "gomel_set_precision_schedule": (ctypes.c_int, [_vp, ctypes.c_int32]),
     "gomel_auto_fp64_iterations": (ctypes.c_int32, [_cfg_p, ctypes.c_int32]),
     "gomel_get_precision": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.POINTER(ctypes.c_int32)]),
+    "gomel_cache_frame_bytes": (ctypes.c_size_t, [_cfg_p, ctypes.c_int, ctypes.c_int]),
+    "gomel_cache_create": (ctypes.c_int, [_vp, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]),
+    "gomel_cache_destroy": (ctypes.c_int, [_vp]),
+    "gomel_cache_write": (ctypes.c_int, [_vp, ctypes.c_int, _vp, ctypes.c_size_t, ctypes.c_size_t, _vp, ctypes.c_size_t, _vp, ctypes.c_size_t, _vp]),
+    "gomel_cache_read": (ctypes.c_int, [_vp, ctypes.c_int, _vp, ctypes.c_size_t, ctypes.c_size_t, _vp, ctypes.c_size_t, ctypes.c_double, ctypes.c_uint64,
+                                        ctypes.c_uint64, _vp]),
+    "gomel_cache_bad_slots": (ctypes.c_int, [_vp, c_u64_p]),
+    "gomel_batch_upload_cache": (ctypes.c_int, [_vp, _vp, _vp, ctypes.POINTER(c_double_p), c_u64_p, _vp]),
+    "gomel_to_mel_cache": (ctypes.c_int, [_vp, ctypes.c_size_t, ctypes.POINTER(c_double_p), c_size_p, _vp, _vp, ctypes.c_size_t, _vp]),
+    "gomel_dropout": (ctypes.c_int, [_vp, ctypes.c_int, _vp, ctypes.c_size_t, _vp, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_double,
+                                     ctypes.c_uint64, ctypes.c_uint64, _vp]),
+    "gomel_dropout_backward": (ctypes.c_int, [_vp, ctypes.c_int, _vp, ctypes.c_size_t, _vp, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_size_t, ctypes.c_double,
+                                              ctypes.c_uint64, ctypes.c_uint64, _vp]),
     "gomel_to_mel_pairs": (ctypes.c_size_t, [_cfg_p, ctypes.c_size_t]),
     "gomel_to_mel": (ctypes.c_int, [_vp, c_double_p, ctypes.c_size_t, c_double_p, ctypes.c_size_t, c_size_p]),
     "gomel_phase_pairs": (ctypes.c_size_t, [_cfg_p, ctypes.c_int32, ctypes.c_size_t]),

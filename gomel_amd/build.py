@@ -1,4 +1,4 @@
-"""Builds libgomel_hip.so (the C-ABI library) in-tree: the HIP translation unit (kernels, launches, device entry points) with hipcc
+"""Builds libgomel_hip.so (the C-ABI library) in-tree: the HIP translation units (kernels, launches, device entry points) with hipcc
 for gfx950, the device-free host logic (csrc/gomel_host.cpp: table builder, schedule, planners, registry, host-only entry points) with
 g++ as plain C++17, linked into one shared object.  `python -m gomel_amd.build [--force]`."""
 import os
@@ -10,8 +10,9 @@ import tempfile
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SRC = os.path.join(CSRC, "gomel_hip.hip")
+CACHE_SRC = os.path.join(CSRC, "gl_cache.hip")
 HOST_SRC = os.path.join(CSRC, "gomel_host.cpp")
-DEPS = [SRC, HOST_SRC] + [os.path.join(CSRC, n) for n in ("gomel_host.hpp", "gl_types.hpp", "gl_fft.hpp", "gl_kernels.hpp", "gl_any.hpp", "gl_big.hpp")] + [
+DEPS = [SRC, CACHE_SRC, HOST_SRC] + [os.path.join(CSRC, n) for n in ("gomel_host.hpp", "gl_cache.hpp", "gl_types.hpp", "gl_fft.hpp", "gl_kernels.hpp", "gl_any.hpp", "gl_big.hpp")] + [
     os.path.join(HERE, "..", "include", "gomel_hip.h")]
 OUT = os.path.join(HERE, "libgomel_hip.so")
 # -target-feature -load-store-opt: switches off the SI load/store optimizer for the device code.  It merges neighbouring
@@ -19,6 +20,8 @@ OUT = os.path.join(HERE, "libgomel_hip.so")
 # wave-instruction, MI355X_MICROARCH.md "LDS"); 66 of the 90 LDS reads per frame of k_gl_fused were merged that way.  The
 # host pass of hipcc does not know the feature and says so in a warning (-Wno-... has no switch for it): harmless.
 HIP_FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Xclang", "-target-feature", "-Xclang", "-load-store-opt"]
+# gl_cache.hip (spectrogram cache, dropout): no packed fp32 instructions; some of their forms have given wrong results on this hardware.
+CACHE_FLAGS = ["-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
 
 
@@ -50,13 +53,14 @@ def build(force=False, verbose=False, out=OUT, extra_flags=()):
     if not force and not extra_flags and not needs_build(out):
         return out
     with tempfile.TemporaryDirectory(prefix="gomel_build_") as tmp:
-        host_o, hip_o = os.path.join(tmp, "gomel_host.o"), os.path.join(tmp, "gomel_hip.o")
+        host_o, hip_o, cache_o = (os.path.join(tmp, n) for n in ("gomel_host.o", "gomel_hip.o", "gl_cache.o"))
         cxx = shutil.which("g++") or shutil.which("c++")
         host_cmd = ([cxx] if cxx else [hipcc(), "-x", "c++"]) + HOST_FLAGS + list(extra_flags) + ["-c", HOST_SRC, "-o", host_o]   # (no g++: the host pass of hipcc's clang)
         if verbose:
             print(" ".join(host_cmd), file=sys.stderr)
         host = subprocess.Popen(host_cmd, stderr=subprocess.PIPE, text=True)                 # beside the device compile
         try:
+            _run([hipcc()] + CACHE_FLAGS + list(extra_flags) + ["-c", CACHE_SRC, "-o", cache_o], verbose)
             _run([hipcc()] + HIP_FLAGS + list(extra_flags) + ["-c", SRC, "-o", hip_o], verbose)
             _, host_err = host.communicate()
             if host_err.strip():
@@ -67,7 +71,7 @@ def build(force=False, verbose=False, out=OUT, extra_flags=()):
             if host.poll() is None:        # the device compile failed: do not leave the host compile writing into a directory that is about to go
                 host.kill()
                 host.communicate()
-        _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out + ".tmp", hip_o, host_o], verbose)
+        _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out + ".tmp", hip_o, cache_o, host_o], verbose)
     os.replace(out + ".tmp", out)
     return out
 

@@ -19,10 +19,11 @@
 
 #include "../../include/gomel_hip.h"
 #include "gomel_host.hpp"
+#include "gl_cache.hpp"
 #include "gl_kernels.hpp"
 
 // =============================================================================================== host side
-static thread_local int g_last_hip = 0;
+thread_local int g_last_hip = 0;
 #define HIPCHK(expr)                                         \
     do {                                                     \
         hipError_t e_ = (expr);                              \
@@ -95,6 +96,22 @@ struct gomel_handle {
 };
 
 constexpr int kErrSlots = 256;
+
+// what the spectrogram cache and dropout (gl_cache.hip) need of a handle
+int handle_device(const gomel_handle* h) { return h->device; }
+int handle_num_mels(const gomel_handle* h) { return h->cfg.num_mels; }
+hipError_t handle_stage(gomel_handle* h, size_t bytes, void** p) { std::lock_guard<std::mutex> lk(h->mu); return (hipError_t)h->pool.alloc(p, bytes); }
+void handle_unstage(gomel_handle* h, void* p) { std::lock_guard<std::mutex> lk(h->mu); h->pool.release(p); }
+
+// Queues `s` behind what is queued on the caller's stream.
+static hipError_t follow(hipStream_t s, hipStream_t caller) {
+    hipEvent_t ev = nullptr;
+    hipError_t e = hipEventCreateWithFlags(&ev, hipEventDisableTiming);
+    if (e == hipSuccess) e = hipEventRecord(ev, caller);
+    if (e == hipSuccess) e = hipStreamWaitEvent(s, ev, 0);
+    if (ev) (void)hipEventDestroy(ev);
+    return e;
+}
 
 // fp64 iterations of a call of I iterations on this handle: 0 = fp32 throughout, >= I = fp64 throughout.  Caller holds h->mu.
 static int resolve_fp64_iterations(const gomel_handle* h, int I) {
@@ -1354,14 +1371,15 @@ static int batch_create_f32_guarded(gomel_handle* h, size_t n_utt, const size_t*
     return batch_create_common(h, n_utt, n_pairs, BF_IO32, -1, out);
 }
 
-// H2D of log-mel and x0 on `st` (asynchronous when the host buffers are pinned).  Pointers are to esz-byte elements.
+// H2D of log-mel and x0 on `st` (asynchronous when the host buffers are pinned).  Pointers are to esz-byte elements; mel null: d_mel
+// has been filled already (batch_upload_cache_guarded).
 static int batch_upload_impl(gomel_batch* b, const void* const* mel, const void* const* x0, const uint64_t* seeds, bool pin_here, bool wait,
                              hipStream_t st) {
     gomel_handle* h = b->h;
     const size_t esz = b->esz;
     b->any_x0 = false;
     for (size_t u = 0; u < b->n_utt; u++) {
-        if (!mel[u]) return GOMEL_ERR_NULL;
+        if (mel && !mel[u]) return GOMEL_ERR_NULL;
         b->utts[u].has_x0 = (x0 && x0[u]) ? 1 : 0;
         b->utts[u].seed = seeds ? seeds[u] : (uint64_t)u;
         b->any_x0 |= b->utts[u].has_x0 != 0;
@@ -1371,13 +1389,13 @@ static int batch_upload_impl(gomel_batch* b, const void* const* mel, const void*
     const size_t row = b->direct ? istft_row(h->cfg.resolut) : 2;   // elements per input unit (magnitude row / pair)
     if (pin_here)
         for (size_t u = 0; u < b->n_utt; u++) {
-            pins.want(mel[u], b->n_pairs[u] * row * esz);
+            if (mel) pins.want(mel[u], b->n_pairs[u] * row * esz);
             if (b->utts[u].has_x0) pins.want(x0[u], (size_t)b->utts[u].len * esz);
         }
     pins.commit(st);
     int64_t poff = 0;
     for (size_t u = 0; u < b->n_utt; u++) {
-        HIPCHK(hipMemcpyAsync((char*)b->d_mel + (size_t)poff * row * esz, mel[u], b->n_pairs[u] * row * esz, hipMemcpyDefault, st));
+        if (mel) HIPCHK(hipMemcpyAsync((char*)b->d_mel + (size_t)poff * row * esz, mel[u], b->n_pairs[u] * row * esz, hipMemcpyDefault, st));
         poff += (int64_t)b->n_pairs[u];
         if (b->utts[u].has_x0)
             HIPCHK(hipMemcpyAsync((char*)b->d_x0 + (size_t)b->utts[u].xoff * esz, x0[u], (size_t)b->utts[u].len * esz, hipMemcpyDefault, st));
@@ -1397,6 +1415,41 @@ static int batch_upload_guarded(gomel_batch* b, const void* const* mel, const vo
     std::lock_guard<std::mutex> lk(b->h->mu);
     DeviceGuard dg(b->h->device); HIPCHK(dg.err);
     return batch_upload_impl(b, mel, x0, seeds, true, true, b->h->stream);
+}
+
+// The spectrograms from a cache: d_mel is the dense output of a read, in the batch's element type.
+static int batch_upload_cache_guarded(gomel_batch* b, gomel_cache* c, const int64_t* slots, const double* const* x0, const uint64_t* seeds, hipStream_t caller) {
+    if (!b || !c || !slots) return GOMEL_ERR_NULL;
+    gomel_handle* h = b->h;
+    if (b->direct || b->io32 || c->l.K != h->cfg.num_mels || c->device != h->device || b->total_frames > (int64_t)kMaxRows) return GOMEL_ERR_BAD_CONFIG;
+    std::lock_guard<std::mutex> lk(h->mu);
+    DeviceGuard dg(h->device); HIPCHK(dg.err);
+    const int kind = memory_kind(slots, h->device);
+    if (kind < 0) return GOMEL_ERR_BAD_CONFIG;
+    const size_t n = (size_t)b->total_frames;
+    if (!kind)
+        for (size_t f = 0; f < n; f++) if (slots[f] < 0 || (uint64_t)slots[f] >= c->n_slots) return GOMEL_ERR_TABLE_RANGE;
+    b->uploaded = false;
+    struct Temp {   // the count of bad slots | the slots, when they come from the host
+        gomel_handle* h; void* p = nullptr;
+        ~Temp() { if (p) { (void)hipStreamSynchronize(h->stream); h->pool.release(p); } }
+    } tmp{h};
+    HIPCHK((hipError_t)h->pool.alloc(&tmp.p, 256 + (kind ? 0 : n * 8)));
+    unsigned long long* bad = (unsigned long long*)tmp.p;
+    const int64_t* at = slots;
+    HIPCHK(follow(h->stream, caller));
+    HIPCHK(hipMemsetAsync(bad, 0, 8, h->stream));
+    if (!kind) {
+        at = (const int64_t*)((char*)tmp.p + 256);
+        HIPCHK(hipMemcpyAsync((void*)at, slots, n * 8, hipMemcpyHostToDevice, h->stream));
+    }
+    const DropRule none{0, 0, 1.0};
+    HIPCHK(cache_read_device(c, GOMEL_F64, b->d_mel, 2 * (size_t)c->l.K, n, at, 0, none, 0, 0, true, bad, h->stream));
+    unsigned long long count = 0;
+    HIPCHK(hipMemcpyAsync(&count, bad, 8, hipMemcpyDeviceToHost, h->stream));
+    HIPCHK(hipStreamSynchronize(h->stream));
+    if (count) return GOMEL_ERR_TABLE_RANGE;
+    return batch_upload_impl(b, nullptr, (const void* const*)x0, seeds, true, true, h->stream);
 }
 
 static int batch_run_guarded(gomel_batch* b) {
@@ -1859,9 +1912,12 @@ static int target_magnitudes_guarded(gomel_handle* h, const double* mel, size_t 
     return rc;
 }
 
+// Where ToMel's frames go instead of the caller's pairs: slots of a cache (device or host memory, in the order of the utterances).
+struct ToCache { gomel_cache* c; const int64_t* slots; size_t n; hipStream_t caller; };
+
 static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* const* wave, const size_t* n_samples, double* const* out_pairs,
-                                const size_t* cap_pairs, size_t* n_pairs_out) {
-    if (!h || !wave || !n_samples || !out_pairs) return GOMEL_ERR_NULL;
+                                const size_t* cap_pairs, size_t* n_pairs_out, const ToCache* into = nullptr) {
+    if (!h || !wave || !n_samples || (!out_pairs && !into)) return GOMEL_ERR_NULL;
     if (n_utt == 0) return GOMEL_ERR_EMPTY;
     const gomel_config& c = h->cfg;
     const int N = c.resolut, H = N / 2, K = c.num_mels, hop = c.window;
@@ -1869,7 +1925,7 @@ static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* con
     std::vector<size_t> P(n_utt), F(n_utt), woff(n_utt), foff(n_utt);
     size_t tot_w = 0, tot_f = 0;
     for (size_t u = 0; u < n_utt; u++) {
-        if (!wave[u] || !out_pairs[u]) return GOMEL_ERR_NULL;
+        if (!wave[u] || (!into && !out_pairs[u])) return GOMEL_ERR_NULL;
         if (n_samples[u] == 0) return GOMEL_ERR_EMPTY;
         P[u] = gomel_pad_len(n_samples[u], hop);                                  // pad, mel/impl.go:429-455
         if (P[u] < (size_t)N) return GOMEL_ERR_TOO_SHORT;
@@ -1883,15 +1939,21 @@ static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* con
     std::vector<int64_t> fx(tot_f);
     for (size_t u = 0; u < n_utt; u++)
         for (size_t f = 0; f < F[u]; f++) fx[foff[u] + f] = (int64_t)(woff[u] + f * (size_t)hop);
+    if (into && into->n != tot_f) return GOMEL_ERR_BAD_LENGTH;
+    if (into && (into->c->l.K != K || into->c->device != h->device || tot_f > kMaxRows)) return GOMEL_ERR_BAD_CONFIG;
     std::lock_guard<std::mutex> lk(h->mu);
     DeviceGuard dg(h->device); HIPCHK(dg.err);
+    const int slots_kind = into ? memory_kind(into->slots, h->device) : 1;
+    if (slots_kind < 0) return GOMEL_ERR_BAD_CONFIG;
+    if (!slots_kind)
+        for (size_t f = 0; f < tot_f; f++) if (into->slots[f] >= 0 && (uint64_t)into->slots[f] >= into->c->n_slots) return GOMEL_ERR_TABLE_RANGE;
     GateOrdinary gate_o; gate_o.enter(h, h->stream);   // synchronous entry point: the gate is left (destructor) after its streams have drained
     double *d_wave = nullptr, *d_smag = nullptr, *d_out = nullptr;
     v2d *d_bigA = nullptr, *d_bigB = nullptr;   // frame lengths above 8192: the convolution's scratch (gl_big.hpp)
     int64_t* d_fx = nullptr;
     int rc = GOMEL_OK;
     PinnedScope pins;                      // big caller buffers: pinned for the call (pageable copies run at a tenth of the rate)
-    for (size_t u = 0; u < n_utt; u++) { pins.want(wave[u], n_samples[u] * 8); pins.want(out_pairs[u], F[u] * (size_t)K * 16); }
+    for (size_t u = 0; u < n_utt; u++) { pins.want(wave[u], n_samples[u] * 8); if (!into) pins.want(out_pairs[u], F[u] * (size_t)K * 16); }
     pins.commit(h->stream, h->copy_stream);
     pins.drain_too(h->up_stream);
     if (h->pool.alloc((void**)&d_wave, tot_w * 8) != hipSuccess || h->pool.alloc((void**)&d_smag, tot_f * (size_t)(H + 1) * 8) != hipSuccess ||
@@ -1902,6 +1964,14 @@ static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* con
         const size_t sc = (size_t)big_chunk_frames(h, (int64_t)tot_f) * (size_t)h->dt.big.Mc * 16;
         if (h->pool.alloc((void**)&d_bigA, sc) != hipSuccess || h->pool.alloc((void**)&d_bigB, sc) != hipSuccess) { g_last_hip = (int)hipGetLastError(); rc = GOMEL_ERR_HIP; }
     }
+    int64_t* d_slots = nullptr;
+    const int64_t* slots = into ? into->slots : nullptr;
+    if (!rc && !slots_kind) {
+        if (h->pool.alloc((void**)&d_slots, tot_f * 8) != hipSuccess) { g_last_hip = (int)hipGetLastError(); rc = GOMEL_ERR_HIP; }
+        else if (hipMemcpyAsync(d_slots, slots, tot_f * 8, hipMemcpyHostToDevice, h->stream) != hipSuccess) rc = GOMEL_ERR_HIP;
+        slots = d_slots;
+    }
+    if (!rc && into && follow(h->stream, into->caller) != hipSuccess) rc = GOMEL_ERR_HIP;
     // Chunks of ~32 MB of samples, pipelined over the handle's three streams as in FromMel's batch call: chunk c+1's waveforms go up
     // while chunk c is transformed and chunk c-1's log-mel comes down (a 256 x 10 s call is H2D-bound: 0.9 GB up, 0.27 GB down,
     // 1.5 ms of kernels -- 28.7 ms one thing after the other, the upload's 18 ms plus a chunk's worth overlapped).  The device
@@ -1939,6 +2009,10 @@ static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* con
                               hipLaunchKernelGGL(k_stft_mag<NN>, dim3((unsigned)((nf + SPB - 1) / SPB)), dim3(128), 0, h->stream, d_wave, d_fx + f0, d_smag + f0 * (size_t)(H + 1), (int64_t)nf, hop, h->dt); });
         if (h->big) hipLaunchKernelGGL(k_domel_log, dim3((unsigned)nf), dim3(256), 0, h->stream, d_smag + f0 * (size_t)(H + 1), h->dt.dom, d_out + f0 * (size_t)K * 2, K, H, 0);
         else hipLaunchKernelGGL(k_domel_log, dim3((unsigned)nf), dim3(256), (size_t)(H + 1) * 8, h->stream, d_smag + f0 * (size_t)(H + 1), h->dt.dom, d_out + f0 * (size_t)K * 2, K, H, 1);
+        if (into) {   // on the compute stream: a slot named twice keeps its last frame across chunks too
+            if (cache_write_device(into->c, GOMEL_F64, d_out + f0 * (size_t)K * 2, 2 * (size_t)K, nf, slots + f0, 0, nullptr, 0, h->stream) != hipSuccess) rc = GOMEL_ERR_HIP;
+            continue;
+        }
         if (hipEventRecord(ev_done[cidx], h->stream) != hipSuccess || hipStreamWaitEvent(h->copy_stream, ev_done[cidx], 0) != hipSuccess) rc = GOMEL_ERR_HIP;
         for (size_t u = u0; u < u1 && !rc; u++)
             if (hipMemcpyAsync(out_pairs[u], d_out + foff[u] * (size_t)K * 2, F[u] * (size_t)K * 16, hipMemcpyDefault, h->copy_stream) != hipSuccess) rc = GOMEL_ERR_HIP;
@@ -1952,6 +2026,7 @@ static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* con
     if (d_smag) h->pool.release(d_smag);
     if (d_out) h->pool.release(d_out);
     if (d_fx) h->pool.release(d_fx);
+    if (d_slots) h->pool.release(d_slots);
     if (d_bigA) h->pool.release(d_bigA);
     if (d_bigB) h->pool.release(d_bigB);
     if (!rc && n_pairs_out) for (size_t u = 0; u < n_utt; u++) n_pairs_out[u] = F[u] * (size_t)K;
@@ -2166,6 +2241,17 @@ int gomel_to_mel(gomel_handle* h, const double* wave, size_t n, double* out_pair
 int gomel_to_mel_batch(gomel_handle* h, size_t n_utt, const double* const* wave, const size_t* n_samples, double* const* out_pairs,
                        const size_t* cap_pairs, size_t* n_pairs_out) {
     GOMEL_TRY return to_mel_batch_guarded(h, n_utt, wave, n_samples, out_pairs, cap_pairs, n_pairs_out); GOMEL_CATCH
+}
+int gomel_batch_upload_cache(gomel_batch* b, gomel_cache* c, const int64_t* slots, const double* const* x0, const uint64_t* seeds, void* stream) {
+    GOMEL_TRY return batch_upload_cache_guarded(b, c, slots, x0, seeds, (hipStream_t)stream); GOMEL_CATCH
+}
+int gomel_to_mel_cache(gomel_handle* h, size_t n_utt, const double* const* wave, const size_t* n_samples, gomel_cache* c, const int64_t* slots,
+                       size_t n_slots_given, void* stream) {
+    if (!c || !slots) return GOMEL_ERR_NULL;
+    GOMEL_TRY
+    const ToCache into{c, slots, n_slots_given, (hipStream_t)stream};
+    return to_mel_batch_guarded(h, n_utt, wave, n_samples, nullptr, nullptr, nullptr, &into);
+    GOMEL_CATCH
 }
 int gomel_to_phase(gomel_handle* h, int32_t num_freqs, const double* wave, size_t n, double* out_pairs, size_t cap_pairs, size_t* n_pairs) {
     GOMEL_TRY return to_phase_guarded(h, num_freqs, wave, n, out_pairs, cap_pairs, n_pairs); GOMEL_CATCH

@@ -38,6 +38,22 @@ int gomel_default_config(gomel_config* c) {
     return GOMEL_OK;
 }
 
+size_t gomel_cache_frame_bytes(const gomel_config* c, int bits, int group_bands) {
+    CacheLayout l;
+    return (c && cache_layout(c->num_mels, bits, group_bands, &l)) ? (size_t)l.row_bytes : 0;
+}
+// Diagnostics (not in the header; the tests reach them by name): the refusal rules of the cache and dropout entry points.
+int gomel_debug_rows_ok(uint64_t a, size_t a_stride, uint64_t b, size_t b_stride, size_t rows, size_t cols, size_t esz) {
+    if (!rows_span(rows, cols, a_stride) || !rows_span(rows, cols, b_stride)) return -1;
+    return rows_disjoint_or_same((const void*)(uintptr_t)a, a_stride, (const void*)(uintptr_t)b, b_stride, rows, cols, esz) ? 1 : 0;
+}
+int gomel_debug_drop_rule(double p, uint32_t* below, int32_t* all, double* scale) {
+    DropRule r;
+    if (!drop_rule(p, &r)) return 0;
+    *below = r.below; *all = r.all; *scale = r.scale;
+    return 1;
+}
+
 size_t gomel_tables_bytes_for(const gomel_config* c) {
     if (validate_config(c) != GOMEL_OK) return 0;
     return sizeof(TableHeader) + (size_t)c->resolut * 8 + ((size_t)c->resolut / 2 + c->num_mels) * sizeof(BinRow);

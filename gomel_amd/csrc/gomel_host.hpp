@@ -91,6 +91,52 @@ struct DevPool {
     }
 };
 
+// ----------------------------------------------------------------------------------------------- spectrogram cache, dropout: host rules
+// How one cached frame lies in memory: the codes (two per pair: 2K bytes at 8 bits, K at 4, channel 0 in the low nibble), padded to 16
+// bytes, then (lo, step) per group as fp32 pairs; the whole padded to 16 bytes so that every row starts on a 16-byte boundary.  Codes and
+// scales share the row because they are always read together: a gathered frame is one run of memory.
+struct CacheLayout {
+    int32_t K, bits, group, groups;   // group: bands per group (0 in the API = K)
+    int64_t scale_off, row_bytes;
+};
+static inline bool cache_layout(int K, int bits, int group_bands, CacheLayout* l) {
+    if (K <= 0 || K > kMaxMels || (bits != 8 && bits != 4)) return false;
+    if (group_bands != 0 && group_bands != 8 && group_bands != 16 && group_bands != 32 && group_bands != 64) return false;
+    l->K = K; l->bits = bits; l->group = group_bands ? group_bands : K;
+    l->groups = (K + l->group - 1) / l->group;
+    l->scale_off = ((int64_t)(bits == 8 ? 2 * K : K) + 15) & ~(int64_t)15;
+    l->row_bytes = (l->scale_off + (int64_t)l->groups * 8 + 15) & ~(int64_t)15;
+    return true;
+}
+static inline int type_bytes(int type) { return type == GOMEL_F64 ? 8 : type == GOMEL_F32 ? 4 : (type == GOMEL_F16 || type == GOMEL_BF16) ? 2 : 0; }
+constexpr size_t kMaxRows = (size_t)INT32_MAX, kMaxElems = (size_t)1 << 56;
+// rows x cols elements `stride` apart: the elements spanned, or 0 where the description is refused
+static inline size_t rows_span(size_t rows, size_t cols, size_t stride) {
+    if (rows == 0 || cols == 0 || stride < cols || rows > kMaxElems || stride > kMaxElems || (rows > 1 && stride > kMaxElems / (rows - 1)) || cols > kMaxElems) return 0;
+    return (rows - 1) * stride + cols;
+}
+// May a kernel read rows x cols at `a` and write rows x cols at `b`?  Yes when they are the same rows (each element is read before it is
+// written, by the same lane), when the spans do not meet, or when rows of one lie in the gaps between rows of the other (columns
+// of one matrix: equal strides, the distance modulo the stride leaves room for `cols` on both sides).
+static inline bool rows_disjoint_or_same(const void* a, size_t a_stride, const void* b, size_t b_stride, size_t rows, size_t cols, size_t esz) {
+    const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
+    if (pa == pb) return a_stride == b_stride || rows == 1;
+    const size_t sa = rows_span(rows, cols, a_stride) * esz, sb = rows_span(rows, cols, b_stride) * esz;
+    if (pa + sa <= pb || pb + sb <= pa) return true;
+    if (a_stride != b_stride) return false;
+    const size_t gap = (pa < pb ? pb - pa : pa - pb) % (a_stride * esz);
+    return gap >= cols * esz && gap <= (a_stride - cols) * esz;
+}
+// 0 <= p <= 1 as (threshold of the 32 random bits, factor of what is kept); false: refused (NaN included)
+struct DropRule { uint32_t below; int32_t all; double scale; };   // drop iff all || u < below
+static inline bool drop_rule(double p, DropRule* r) {
+    if (!(p >= 0.0 && p <= 1.0)) return false;
+    const double t = std::nearbyint(p * 4294967296.0);
+    r->all = t >= 4294967296.0; r->below = r->all ? 0xFFFFFFFFu : (uint32_t)t;
+    r->scale = r->all ? 0.0 : 1.0 / (1.0 - p);
+    return true;
+}
+
 // ----------------------------------------------------------------------------------------------- tables, schedule
 static double hz_to_mel(double v) { return 1127.0 * std::log(1.0 + (v / 700.0)); }  // mel/impl.go:304-308
 static double mel_to_hz(double v) { return 700.0 * (std::exp(v / 1127.0) - 1.0); }  // mel/impl.go:298-302

@@ -23,14 +23,14 @@ class ErrFileNotLoaded(Exception):
 
 
 class DevicePointer:
-    """`numel` float64 elements in the memory of the handle's device at address `ptr` (from hipMalloc, another library, a pipeline stage
-    that keeps its spectrograms in HBM): what the batch calls take wherever they take an array (include/gomel_hip.h "Pointers").  The
-    caller owns the memory and must have finished writing it (the library copies on its own streams)."""
+    """`numel` elements (float64 unless `dtype` names another type) in the memory of the handle's device at address `ptr` (from hipMalloc,
+    another library, a pipeline stage that keeps its spectrograms in HBM): what the batch calls take wherever they take an array
+    (include/gomel_hip.h "Pointers").  The caller owns the memory and must have finished writing it (the library copies on its own
+    streams).  The cache and dropout calls also take dtype "float32", "float16", "bfloat16" and, for slots, "int64"."""
     is_cuda = True
-    dtype = "float64"
 
-    def __init__(self, ptr, numel):
-        self._ptr, self._numel = int(ptr), int(numel)
+    def __init__(self, ptr, numel, dtype="float64"):
+        self._ptr, self._numel, self.dtype = int(ptr), int(numel), dtype
 
     def data_ptr(self):
         return self._ptr
@@ -364,6 +364,34 @@ class Engine:
         check(L.gomel_to_mel_batch(self._h, n, ctypes.cast(wp, dpp), ns, ctypes.cast(op, dpp), cp, got), "gomel_to_mel_batch")
         return [o[:g] for o, g in zip(outs, got)]
 
+    # -- spectrogram cache, dropout ------------------------------------------------------------------
+    def cache(self, n_slots, bits=8, group=0):
+        """A device-resident cache of `n_slots` quantised frames of this engine's NumMels (gomel_amd.Cache)."""
+        from .cache import Cache
+        return Cache(self, n_slots, bits, group)
+
+    def to_mel_cache(self, waves, cache, slots, stream=None):
+        """gomel_to_mel_cache: ToMel of every waveform, the frames quantised into `cache` at `slots` (one per frame, in the order of
+        the waveforms).  Returns the number of frames of each waveform."""
+        from .cache import to_mel_cache
+        return to_mel_cache(self, waves, cache, slots, stream)
+
+    def from_cache(self, cache, slots, x0s=None, seeds=None, stream=None):
+        """FromMel of utterances whose frames are held in `cache`: `slots` is one array of slots per utterance.  Returns the waveforms."""
+        from .cache import from_cache
+        return from_cache(self, cache, slots, x0s, seeds, stream)
+
+    def dropout(self, x, p, seed, offset=0, out=None, stream=None):
+        """gomel_dropout: x with each element dropped (0) with probability `p` or scaled by 1 / (1 - p), by the counter-based generator at
+        (seed, offset + dense index).  A torch tensor that requires a gradient gets one (the mask is made again, never stored)."""
+        from .cache import dropout
+        return dropout(self, x, p, seed, offset, out, stream)
+
+    def dropout_backward(self, dy, p, seed, offset=0, out=None, stream=None):
+        """gomel_dropout_backward: the gradient of `dropout` with the same (p, seed, offset) from the gradient of its output."""
+        from .cache import dropout_backward
+        return dropout_backward(self, dy, p, seed, offset, out, stream)
+
     # -- FFT test hooks ------------------------------------------------------------------------------
     def rfft_frames(self, frames):
         f = np.ascontiguousarray(frames, dtype=np.float32)
@@ -443,8 +471,20 @@ class Batch:
             raise ValueError("mel shapes do not match the batch plan")
         mp = (c_double_p * n)(*[_device_ptr(m, 2 * k, "mel") if _is_device_tensor(m) else m.ctypes.data_as(c_double_p)
                                 for m, k in zip(ms, self.n_pairs)])
-        xp = None
-        xs = None
+        xp, xs, sp = self._x0_args(x0s, seeds)
+        self._keep = (ms, xs)
+        check(_lib.lib().gomel_batch_upload(self._b, mp, xp, sp), "gomel_batch_upload")
+        self._keep = None
+
+    def upload_cache(self, cache, slots, x0s=None, seeds=None, stream=None):
+        """upload with the spectrograms taken from `cache`: `slots` holds one slot per frame of the batch, in order (gomel_batch_upload_cache)."""
+        from .cache import batch_upload_cache
+        batch_upload_cache(self, cache, slots, x0s, seeds, stream)
+
+    def _x0_args(self, x0s, seeds):
+        """(pointer array, keep-alive list, seed array) of an upload."""
+        n = len(self.n_pairs)
+        xp = xs = sp = None
         if x0s is not None:
             xs = [x if (x is None or _is_device_tensor(x)) else np.ascontiguousarray(x, dtype=np.float64) for x in x0s]
             for x, L in zip(xs, self.lens):
@@ -452,12 +492,9 @@ class Batch:
                     raise ValueError("x0 length mismatch")
             xp = (c_double_p * n)(*[None if x is None else (_device_ptr(x, L, "x0") if _is_device_tensor(x) else x.ctypes.data_as(c_double_p))
                                     for x, L in zip(xs, self.lens)])
-        sp = None
         if seeds is not None:
             sp = (ctypes.c_uint64 * n)(*[int(s) & (2 ** 64 - 1) for s in seeds])
-        self._keep = (ms, xs)
-        check(_lib.lib().gomel_batch_upload(self._b, mp, xp, sp), "gomel_batch_upload")
-        self._keep = None
+        return xp, xs, sp
 
     def run(self):
         check(_lib.lib().gomel_batch_run(self._b), "gomel_batch_run")

@@ -264,6 +264,76 @@ int32_t gomel_auto_fp64_iterations(const gomel_config* cfg, int32_t iterations);
  * mode: *fp64_iterations = 0 (fp32 throughout) ... iterations (fp64 throughout). */
 int gomel_get_precision(const gomel_handle* h, int32_t iterations, int32_t* fp64_iterations);
 
+/* ------------------------------------------------------------------------------------------------ spectrogram cache, dropout
+ * Element types of the entry points below. */
+#define GOMEL_F64 0
+#define GOMEL_F32 1
+#define GOMEL_F16 2
+#define GOMEL_BF16 3
+
+/* A device-resident cache of log-mel frames, quantised as they are written and read back dequantised: what the 8-bit image is to a
+ * whole spectrogram on the host (mel/impl.go:127-193: minimum, maximum, 8-bit pixels), frame by frame on the device -- for a model that
+ * generates frames one at a time, for corpora kept in HBM for training, for FromMel (gomel_batch_upload_cache) and from ToMel
+ * (gomel_to_mel_cache).
+ *   A frame is NumMels pairs (2 * NumMels values, the layout of mel_pairs).  `bits` = 8 or 4 per value.  `group_bands` bands (0 = the
+ * whole frame, or 8, 16, 32, 64; both channels of a band belong to its group, the last group may be short) share
+ *     lo   = min of the group's finite values, hi = max, each rounded to fp32 (beyond fp32: the largest fp32 number)
+ *     step = fp32((hi - lo) / (2^bits - 1)), difference and quotient in fp64
+ * and a value x is held as q = rint((x - lo) / step) -- evaluated in fp64, ties to even, clamped to 0 ... 2^bits - 1; 0 where step = 0 --
+ * and reads as lo + q * step: at most half a step from x.  -inf is held as q = 0, +inf as the largest q; a group with no finite
+ * value that is all -inf (all +inf) reads as that; a group that contains a NaN, or both infinities and nothing finite, reads as NaN.
+ *   The cache has `n_slots` slots of one frame (gomel_cache_frame_bytes each, plus 4 bytes); slots never written read as zeros.
+ * Pages, sequences and their tables are the caller's: a call takes `slots`, one int64 per frame (host or device memory), or NULL =
+ * the slots first, first + 1, ...  A negative slot marks padding: nothing is written to the cache, and the frame's row of the output
+ * (`values`, `frames`) is left as it was.  A slot >= n_slots: in host memory the call is refused (GOMEL_ERR_TABLE_RANGE), in device
+ * memory the frame is treated as padding and counted (gomel_cache_bad_slots).  The same slot twice in one write: the later frame is
+ * the one that stays.
+ *   `frames` and `values` are rows of 2 * NumMels elements of `type`, `stride` elements apart (>= 2 * NumMels), in host memory or
+ * memory of the cache's device.  With everything in device memory a call only queues kernels on `stream` (a hipStream_t of that
+ * device; NULL = the default stream) and can be captured into a graph; with anything in host memory it copies through a staging
+ * buffer and returns when it is done (not while `stream` is being captured: GOMEL_ERR_BAD_CONFIG).  Calls that touch the same
+ * slots on different streams are the caller's to order.  `n` = 0 is a call without work.
+ *   gomel_cache_write: quantises n frames.  values != NULL also receives what the cache now stands for, rounded to `type` (what a
+ * generating model is to be conditioned on; the forward of training through the quantiser, whose straight-through gradient is the
+ * identity); values may be frames itself (same stride) but must not overlap it otherwise.
+ *   gomel_cache_read: dequantises n frames (fp32 arithmetic; fp64 for GOMEL_F64), rounded once to `type`.  p > 0 applies dropout
+ * (below) to the values read, element index = position in the dense [n][2 * NumMels] output.
+ * The cache keeps nothing of the handle (its NumMels and device are copied): either may be destroyed first. */
+typedef struct gomel_cache gomel_cache;
+size_t gomel_cache_frame_bytes(const gomel_config* cfg, int bits, int group_bands); /* host only; 0 for arguments that create refuses */
+int gomel_cache_create(gomel_handle* h, size_t n_slots, int bits, int group_bands, gomel_cache** out);
+int gomel_cache_destroy(gomel_cache* c);
+int gomel_cache_write(gomel_cache* c, int type, const void* frames, size_t stride, size_t n, const int64_t* slots, size_t first,
+                      void* values, size_t values_stride, void* stream);
+int gomel_cache_read(gomel_cache* c, int type, void* frames, size_t stride, size_t n, const int64_t* slots, size_t first,
+                     double p, uint64_t seed, uint64_t offset, void* stream);
+/* How many frames were skipped so far because their slot, in device memory, was >= n_slots; counts the calls whose work has finished
+ * (synchronise their streams first) and starts again at zero. */
+int gomel_cache_bad_slots(gomel_cache* c, uint64_t* count);
+/* gomel_batch_upload with the spectrograms taken from a cache of the same NumMels and device: slots[f] for the batch's frames in
+ * order (host or device memory; every one a slot of the cache: padding and slots >= n_slots are refused with GOMEL_ERR_TABLE_RANGE,
+ * and the batch then has to be uploaded again).  Work queued on `stream` before the call is seen.  Returns when the batch is uploaded,
+ * as gomel_batch_upload does. */
+int gomel_batch_upload_cache(gomel_batch* b, gomel_cache* c, const int64_t* slots, const double* const* x0, const uint64_t* seeds, void* stream);
+/* gomel_to_mel_batch into a cache: the log-mel frames never leave the device.  n_slots_given = frames expected (must equal the sum of
+ * gomel_to_mel_pairs / NumMels over the utterances), slots as above, in the order of the utterances.  Returns when they are written;
+ * work queued on `stream` before the call is waited for. */
+int gomel_to_mel_cache(gomel_handle* h, size_t n_utt, const double* const* wave, const size_t* n_samples, gomel_cache* c,
+                       const int64_t* slots, size_t n_slots_given, void* stream);
+
+/* Dropout from a counter-based generator: the mask is never stored, backward makes it again from (p, seed, offset).  Element e =
+ * offset + row * cols + col (mod 2^64) is dropped iff u(e) < rint(p * 2^32), u(e) = the low (e even) or high (e odd) 32 bits of
+ *     splitmix64(seed + (e / 2 + 1) * 0x9E3779B97F4A7C15)
+ * -- the generator of gomel_from_mel's x0.  Forward: y = 0 where dropped (whatever x holds there, a NaN too), x / (1 - p) where kept;
+ * backward: dx = 0 / dy / (1 - p) likewise, so the two are the same operation on other buffers and each has its entry point.  0 <= p <= 1.
+ * `rows` x `cols` elements of `type`, rows x_stride / y_stride elements apart (>= cols), host or device memory, `stream` and capture as
+ * above.  In place (y = x, same stride) is allowed, other overlap is refused (GOMEL_ERR_BAD_CONFIG).  Products are fp32 (fp64 for
+ * GOMEL_F64), rounded once.  Two calls with one seed and disjoint ranges of e draw independent masks. */
+int gomel_dropout(gomel_handle* h, int type, const void* x, size_t x_stride, void* y, size_t y_stride, size_t rows, size_t cols,
+                  double p, uint64_t seed, uint64_t offset, void* stream);
+int gomel_dropout_backward(gomel_handle* h, int type, const void* dy, size_t dy_stride, void* dx, size_t dx_stride, size_t rows, size_t cols,
+                           double p, uint64_t seed, uint64_t offset, void* stream);
+
 /* (*Mel).ToMel, mel/mel.go:46-74 = pad + gossp STFT + |S[j]|,|S[N-1-j]| + domel + ln(max(v,1e-5)). */
 size_t gomel_to_mel_pairs(const gomel_config* cfg, size_t n_samples);
 int gomel_to_mel(gomel_handle* h, const double* wave, size_t n_samples, double* out_pairs, size_t cap_pairs,

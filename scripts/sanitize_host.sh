@@ -31,7 +31,8 @@ if [ -z "$GOMEL_SAN_HOST_ONLY" ] && command -v hipcc > /dev/null; then
   RT=$(dirname $($CLANG -print-file-name=libclang_rt.asan-x86_64.so))
   run $CLANG $COMMON $SAN -shared-libasan -c gomel_amd/csrc/gomel_host.cpp -o $OUT/asan/gomel_host.o
   run hipcc -O1 -g --offload-arch=gfx950 -fno-gpu-sanitize -std=c++17 -fPIC -fno-omit-frame-pointer -w -Xclang -target-feature -Xclang -load-store-opt $SAN -shared-libasan -c gomel_amd/csrc/gomel_hip.hip -o $OUT/asan/gomel_hip.o
-  run hipcc --offload-arch=gfx950 -shared -fPIC $SAN -shared-libasan -o $OUT/asan/libgomel_hip.so $OUT/asan/gomel_hip.o $OUT/asan/gomel_host.o
+  run hipcc -O1 -g --offload-arch=gfx950 -fno-gpu-sanitize -std=c++17 -fPIC -fno-omit-frame-pointer -w -Xclang -target-feature -Xclang -packed-fp32-ops $SAN -shared-libasan -c gomel_amd/csrc/gl_cache.hip -o $OUT/asan/gl_cache.o
+  run hipcc --offload-arch=gfx950 -shared -fPIC $SAN -shared-libasan -o $OUT/asan/libgomel_hip.so $OUT/asan/gomel_hip.o $OUT/asan/gl_cache.o $OUT/asan/gomel_host.o
   LD_PRELOAD=$RT/libclang_rt.asan-x86_64.so ASAN_OPTIONS=detect_leaks=0 UBSAN_OPTIONS=print_stacktrace=1 GOMEL_LIB=$OUT/asan/libgomel_hip.so \
       run python3 -m pytest tests/test_abi.py tests/test_tables.py tests/test_chunk_plan.py tests/test_dist.py -q -p no:cacheprovider -k "not links_from_c and not gloo"   # (the gcc-built C caller cannot link a clang-ASan library; the normal suite runs it)
 fi
