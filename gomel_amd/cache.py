@@ -10,50 +10,75 @@ import numpy as np
 
 from . import _lib
 from ._lib import check
-from .mel import Batch, DevicePointer, _is_device_tensor
+from .mel import Batch, DevicePointer
 
 _TYPES = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}
-_torch_types = {}
+_torch = None                # the module, once a tensor has been seen
+_Tensor = None               # its Tensor type
+_torch_types, _int64 = {}, None
+_raw_stream = None           # device index -> hipStream_t of torch's current stream
 
 
-def _torch_type(dtype):
-    """The element type's code of a torch dtype, None for one the library does not take."""
-    if not _torch_types:
-        import torch
-        _torch_types.update({torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3})
-    return _torch_types.get(dtype)
+def _is_tensor(a):
+    """Whether `a` is a torch tensor (torch is never imported for the question)."""
+    global _torch, _Tensor, _int64, _raw_stream
+    if _Tensor is not None:
+        return isinstance(a, _Tensor)
+    if "torch" not in sys.modules or not hasattr(a, "data_ptr") or isinstance(a, DevicePointer):
+        return False
+    import torch
+    _torch_types.update({torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3})
+    _int64 = torch.int64
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    _torch, _Tensor = torch, torch.Tensor
+    return isinstance(a, _Tensor)
 
 
-def _stream(stream, *arrays):
+def _stream(stream, device):
     """The hipStream_t a call runs on: `stream` (an integer handle, or an object with .cuda_stream), else torch's current stream of the
-    first torch tensor's device, else the default stream."""
+    tensors' device, else the default stream."""
     if stream is not None:
         return int(getattr(stream, "cuda_stream", stream))
-    for a in arrays:
-        if a is not None and not isinstance(a, (np.ndarray, DevicePointer)):
-            import torch
-            return torch.cuda.current_stream(a.device).cuda_stream
-    return 0
+    return 0 if device is None else _raw_stream(device)
+
+
+def _device_of(engine_device, *devices):
+    """The device of a call's tensors (None: there are none); they have to be on one device, the engine's."""
+    got = None
+    for d in devices:
+        if d is not None:
+            if (got is not None and d != got) or (engine_device >= 0 and d != engine_device):
+                raise ValueError("a tensor on device %d was handed to a call on device %d" % (d, engine_device if engine_device >= 0 else got))
+            got = d
+    return got
 
 
 def _rows(a, cols, what, write=False):
-    """(address, type code, row stride in elements, rows) of an array of rows of `cols` elements.  Rows may be apart; the elements of
-    a row are consecutive."""
-    if isinstance(a, DevicePointer):
+    """(address, type code, row stride in elements, rows, device) of an array of rows of `cols` elements.  Rows may be apart; the
+    elements of a row are consecutive.  device: a torch tensor's, None otherwise."""
+    device = None
+    if _is_tensor(a):
+        device, t = a.get_device(), _torch_types.get(a.dtype)
+        if device < 0 or not a.is_cuda:
+            raise ValueError("%s: a torch tensor must be on the GPU (numpy arrays are taken from host memory)" % what)
+        if t is not None and a.is_contiguous():
+            rows, rest = divmod(a.numel(), cols)
+            if not rest:
+                return a.data_ptr(), t, cols, rows, device
+        strides, ptr = a.stride(), a.data_ptr()
+    elif isinstance(a, DevicePointer):
         t, n = _TYPES.get(a.dtype), a.numel()
         if t is None or n % cols:
             raise ValueError("%s: a DevicePointer of float64 / float32 / float16 / bfloat16 with whole rows of %d elements is needed" % (what, cols))
-        return a.data_ptr(), t, cols, n // cols
-    if isinstance(a, np.ndarray):
+        return a.data_ptr(), t, cols, n // cols, None
+    elif isinstance(a, np.ndarray):
         t, strides, ptr = _TYPES.get(a.dtype.name), [s // a.itemsize for s in a.strides], a.ctypes.data
         if any(s % a.itemsize for s in a.strides) or not a.dtype.isnative:
             t = None
         if write and not a.flags.writeable:
             raise ValueError("%s: the array is read-only" % what)
     elif hasattr(a, "data_ptr"):
-        if not a.is_cuda:
-            raise ValueError("%s: a torch tensor must be on the GPU (numpy arrays are taken from host memory)" % what)
-        t, strides, ptr = _torch_type(a.dtype), a.stride(), a.data_ptr()
+        raise ValueError("%s: a torch tensor must be on the GPU (numpy arrays are taken from host memory)" % what)
     else:
         raise TypeError("%s: a numpy array, a torch CUDA tensor or a DevicePointer is needed, not %s" % (what, type(a).__name__))
     if t is None:
@@ -62,11 +87,11 @@ def _rows(a, cols, what, write=False):
     n = 1
     for s in shape:
         n *= s
-    if n % cols or n == 0 and cols == 0:
+    if n % cols:
         raise ValueError("%s: whole rows of %d elements are needed, not shape %s" % (what, cols, shape))
     rows = n // cols
     if rows == 0:
-        return ptr, t, cols, 0
+        return ptr, t, cols, 0, device
     # innermost dimensions that make up one row have to be dense; what remains has to step evenly from row to row
     inner, i = 1, len(shape)
     while inner < cols:
@@ -79,7 +104,7 @@ def _rows(a, cols, what, write=False):
                 raise ValueError("%s: whole rows of %d elements are needed, not shape %s" % (what, cols, shape))
             if inner != n:
                 raise ValueError("%s: rows of %d elements cannot be stepped through evenly" % (what, cols))
-            return ptr, t, cols, rows
+            return ptr, t, cols, rows, device
     step, count = None, 1
     for k in range(i - 1, -1, -1):
         if shape[k] == 1:
@@ -94,33 +119,27 @@ def _rows(a, cols, what, write=False):
         step = cols
     if step < cols:
         raise ValueError("%s: rows overlap" % what)
-    return ptr, t, step, rows
+    return ptr, t, step, rows, device
 
 
 def _slots(slots, n, what="slots"):
-    """(address, the array that has to stay alive) of one int64 per frame."""
+    """(address, the array that has to stay alive, device) of one int64 per frame."""
+    if _is_tensor(slots):
+        device = slots.get_device()
+        if device < 0 or slots.dtype != _int64 or not slots.is_contiguous() or slots.numel() != n:
+            raise ValueError("%s: a contiguous int64 CUDA tensor with %d elements is needed" % (what, n))
+        return slots.data_ptr(), slots, device
     if isinstance(slots, DevicePointer):
         if slots.dtype != "int64" or slots.numel() != n:
             raise ValueError("%s: a DevicePointer of %d int64 is needed" % (what, n))
-        return slots.data_ptr(), slots
-    if hasattr(slots, "data_ptr"):
-        if not slots.is_cuda or str(slots.dtype) != "torch.int64" or not slots.is_contiguous() or slots.numel() != n:
-            raise ValueError("%s: a contiguous int64 CUDA tensor with %d elements is needed" % (what, n))
-        return slots.data_ptr(), slots
+        return slots.data_ptr(), slots, None
     a = np.asarray(slots)
     if a.dtype.kind not in "iu" and a.size:
         raise ValueError("%s: integers are needed, not %s" % (what, a.dtype))
     a = np.ascontiguousarray(a, dtype=np.int64).reshape(-1)
     if a.size != n:
         raise ValueError("%s: one slot per frame is needed (%d frames, %d slots)" % (what, n, a.size))
-    return (a.ctypes.data if n else 0), a
-
-
-def _same_device(engine_device, *arrays):
-    for a in arrays:
-        if a is not None and not isinstance(a, (np.ndarray, DevicePointer)) and hasattr(a, "device") and engine_device >= 0:
-            if a.device.index != engine_device:
-                raise ValueError("a tensor on %s was handed to an engine on device %d" % (a.device, engine_device))
+    return (a.ctypes.data if n else 0), a, None
 
 
 class Cache:
@@ -143,17 +162,16 @@ class Cache:
         """Quantises `frames` ([n, NumMels, 2] or [n * NumMels, 2]) into their slots.  `values` (same shape and type; may be `frames` itself)
         receives what the cache now stands for, and is returned."""
         cols = 2 * self.num_mels
-        ptr, t, stride, n = _rows(frames, cols, "frames")
-        sp, keep = (0, None) if slots is None else _slots(slots, n)
-        vp, vs = 0, cols
+        ptr, t, stride, n, dev = _rows(frames, cols, "frames")
+        sp, keep, sdev = (0, None, None) if slots is None else _slots(slots, n)
+        vp, vs, vdev = 0, cols, None
         if values is not None:
-            vp, vt, vs, vn = _rows(values, cols, "values", write=True)
+            vp, vt, vs, vn, vdev = _rows(values, cols, "values", write=True)
             if vt != t or vn != n:
                 raise ValueError("values: the frames' type and number of frames are needed")
         if first < 0:
             raise ValueError("first is negative")
-        _same_device(self.device, frames, values, slots)
-        rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, frames, values, keep))
+        rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, _device_of(self.device, dev, vdev, sdev)))
         if rc:
             check(rc, "gomel_cache_write")
         return values
@@ -161,12 +179,12 @@ class Cache:
     def read(self, out, slots=None, first=0, p=0.0, seed=0, offset=0, stream=None):
         """Dequantises frames into `out` ([n, NumMels, 2] or [n * NumMels, 2]) and returns it.  p > 0: with dropout, as Engine.dropout of
         the dense result."""
-        ptr, t, stride, n = _rows(out, 2 * self.num_mels, "out", write=True)
-        sp, keep = (0, None) if slots is None else _slots(slots, n)
+        ptr, t, stride, n, dev = _rows(out, 2 * self.num_mels, "out", write=True)
+        sp, keep, sdev = (0, None, None) if slots is None else _slots(slots, n)
         if first < 0:
             raise ValueError("first is negative")
-        _same_device(self.device, out, slots)
-        rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, out, keep))
+        rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
+                        _stream(stream, _device_of(self.device, dev, sdev)))
         if rc:
             check(rc, "gomel_cache_read")
         return out
@@ -191,19 +209,18 @@ class Cache:
 
 # ------------------------------------------------------------------------------------------------ FromMel / ToMel and the cache
 def batch_upload_cache(batch, cache, slots, x0s=None, seeds=None, stream=None):
-    sp, keep = _slots(slots, sum(batch.n_pairs) // batch.engine.cfg.num_mels)
+    sp, keep, dev = _slots(slots, sum(batch.n_pairs) // batch.engine.cfg.num_mels)
     xp, xs, seed_p = batch._x0_args(x0s, seeds)
-    check(_lib.lib().gomel_batch_upload_cache(batch._b, cache._c, sp, xp, seed_p, _stream(stream, keep)), "gomel_batch_upload_cache")
-    del xs
+    check(_lib.lib().gomel_batch_upload_cache(batch._b, cache._c, sp, xp, seed_p, _stream(stream, _device_of(cache.device, dev))), "gomel_batch_upload_cache")
+    del xs, keep
 
 
 def from_cache(engine, cache, slots, x0s=None, seeds=None, stream=None):
     counts = [int(s.numel()) if hasattr(s, "numel") else len(s) for s in slots]
     if not counts:
         return []
-    if any(_is_device_tensor(s) for s in slots):
-        import torch
-        flat = torch.cat([s.reshape(-1) for s in slots])
+    if any(_is_tensor(s) for s in slots):
+        flat = _torch.cat([s.reshape(-1) for s in slots])
     else:
         flat = np.concatenate([np.asarray(s, dtype=np.int64).reshape(-1) for s in slots])
     b = Batch(engine, [c * engine.cfg.num_mels for c in counts])
@@ -220,51 +237,47 @@ def to_mel_cache(engine, waves, cache, slots, stream=None):
     ws = [np.ascontiguousarray(w, dtype=np.float64) for w in waves]
     counts = [L.gomel_to_mel_pairs(ctypes.byref(engine.cfg), w.size) // engine.cfg.num_mels for w in ws]
     total = sum(counts)
-    sp, keep = _slots(slots, total)
+    sp, keep, dev = _slots(slots, total)
     wp = (_lib.c_double_p * len(ws))(*[w.ctypes.data_as(_lib.c_double_p) for w in ws])
     ns = (ctypes.c_size_t * len(ws))(*[w.size for w in ws])
-    check(L.gomel_to_mel_cache(engine._h, len(ws), wp, ns, cache._c, sp, total, _stream(stream, keep)), "gomel_to_mel_cache")
+    check(L.gomel_to_mel_cache(engine._h, len(ws), wp, ns, cache._c, sp, total, _stream(stream, _device_of(cache.device, dev))), "gomel_to_mel_cache")
+    del keep
     return counts
 
 
 # ------------------------------------------------------------------------------------------------ dropout
 def _flat(a, what, write=False):
-    """(address, type code, row stride, rows, cols) of any array that is dense, or whose rows (its last dimension) are."""
-    if isinstance(a, DevicePointer):
-        ptr, t, _, _ = _rows(a, 1, what, write)
-        return ptr, t, a.numel(), 1, a.numel()
-    n = 1
-    for s in a.shape:
-        n *= s
-    dense = a.flags.c_contiguous if isinstance(a, np.ndarray) else (a.is_contiguous() if hasattr(a, "is_contiguous") else False)
+    """(address, type code, row stride, rows, cols, device) of any array that is dense, or whose rows (its last dimension) are."""
+    if _is_tensor(a):
+        n, dense = a.numel(), a.is_contiguous()
+    elif isinstance(a, np.ndarray):
+        n, dense = a.size, a.flags.c_contiguous
+    else:
+        n, dense = (a.numel() if isinstance(a, DevicePointer) else 1), True
     if dense or n == 0:
-        ptr, t, _, _ = _rows(a, max(n, 1), what, write) if n else _rows(a, 1, what, write)
-        return ptr, t, n, 1, n
+        ptr, t, _, _, device = _rows(a, n or 1, what, write)
+        return ptr, t, n, 1, n, device
     cols = int(a.shape[-1])
-    ptr, t, stride, rows = _rows(a, cols, what, write)
-    return ptr, t, stride, rows, cols
+    ptr, t, stride, rows, device = _rows(a, cols, what, write)
+    return ptr, t, stride, rows, cols, device
 
 
 def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
-    ptr, t, xs, rows, cols = _flat(x, "x")
+    ptr, t, xs, rows, cols, dev = _flat(x, "x")
     if out is None:
         if isinstance(x, DevicePointer):
             raise ValueError("out: a DevicePointer needs one")
-        if isinstance(x, np.ndarray):
-            out = np.empty(x.shape, x.dtype)
-        else:
-            import torch
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    optr, ot, os_, orows, ocols = _flat(out, "out", write=True)
+        out = np.empty(x.shape, x.dtype) if dev is None else _torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    optr, ot, os_, orows, ocols, odev = _flat(out, "out", write=True)
     if ot != t or getattr(out, "shape", None) != getattr(x, "shape", None) or rows * cols != orows * ocols:
         raise ValueError("out: x's type and shape are needed")
-    if (rows, cols) != (orows, ocols):       # one of the two is dense: walk it by the other's rows
+    if rows != orows:                        # one of the two is dense: walk it by the other's rows
         if rows == 1:
             rows, cols, xs = orows, ocols, ocols
         else:
             os_ = cols
-    _same_device(int(engine.cfg.device), x, out)
-    rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, x, out))
+    rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
+            _stream(stream, _device_of(engine.cfg.device, dev, odev)))
     if rc:
         check(rc, where)
     return out
@@ -296,7 +309,7 @@ def _dropout_function():
 
 
 def _wants_grad(x):
-    return "torch" in sys.modules and getattr(x, "requires_grad", False) and sys.modules["torch"].is_grad_enabled()
+    return getattr(x, "requires_grad", False) and sys.modules["torch"].is_grad_enabled()
 
 
 def dropout(engine, x, p, seed, offset=0, out=None, stream=None):

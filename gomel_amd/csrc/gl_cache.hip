@@ -41,25 +41,99 @@ GL_DEV Scale group_scale(double mn, double mx, int flags, int levels) {
     const float lo = to_f32(mn), hi = to_f32(mx);
     return Scale{lo, (float)(((double)hi - (double)lo) / (double)levels)};
 }
-// fp64 because neighbouring codes meet at borders that fp32 quotients step over: 1 value in 3e4 would get the other code.
-GL_DEV int quantise(double v, Scale s, int levels) {
-    if (!(s.step > 0.0f)) return 0;
-    const double q = rint((v - (double)s.lo) / (double)s.step);
-    return (int)fmin(fmax(q, 0.0), (double)levels);
+// The code of v as a number.  In fp64, because neighbouring codes meet at borders that fp32 quotients step over (1 value in 3e4 would get
+// the other code).  `per` = 1 / step (0 where step is 0): the product is within 1e-13 of the quotient, so only a value that close to
+// a border -- and beside it, with room -- needs the division itself.  NaN and infinities: fmaxf / fminf return the number.
+GL_DEV float quantise(double v, Scale s, double per, float levels) {
+    const double d = v - (double)s.lo;
+    double t = d * per, q = rint(t);
+    if (fabs(t - q) > 0.5 - 1e-10) q = rint(d / (double)s.step);
+    return fminf(fmaxf((float)q, 0.0f), levels);
 }
-GL_DEV float dequantise(int q, Scale s, float) { return fmaf((float)q, s.step, s.lo); }
-GL_DEV double dequantise(int q, Scale s, double) { return fma((double)q, (double)s.step, (double)s.lo); }
+GL_DEV float dequantise(float q, Scale s, float) { return fmaf(q, s.step, s.lo); }
+GL_DEV double dequantise(float q, Scale s, double) { return fma((double)q, (double)s.step, (double)s.lo); }
 
 // ------------------------------------------------------------------------------------------------ the generator
-GL_DEV uint64_t splitmix(uint64_t seed, uint64_t i) {   // the word of x0's sample i (k_init_x)
-    uint64_t z = seed + (i + 1) * 0x9E3779B97F4A7C15ull;
+constexpr uint64_t kGamma = 0x9E3779B97F4A7C15ull;
+GL_DEV uint64_t splitmix_of(uint64_t z) {   // the word of x0's sample i (k_init_x): z = seed + (i + 1) * kGamma
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
     return z ^ (z >> 31);
 }
-GL_DEV bool dropped(const DropRule& r, uint64_t seed, uint64_t e) {
-    const uint64_t w = splitmix(seed, e >> 1);
-    return r.all || (uint32_t)((e & 1) ? w >> 32 : w) < r.below;
+
+// ------------------------------------------------------------------------------------------------ 16-byte units
+// A lane moves 16 bytes of frames or activations at a time: UV values of T.  Rows may start at any element (gfx950 takes a 16-byte access
+// at any element's alignment), a row's last unit may be partial.
+template <class T> constexpr int UV = 16 / (int)sizeof(T);
+typedef uint32_t raw_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t raw_word __attribute__((ext_vector_type(4), aligned(4)));
+template <class T> struct Raw { typedef raw_word type; };
+template <> struct Raw<__half> { typedef raw_any type; };
+template <> struct Raw<__hip_bfloat16> { typedef raw_any type; };
+template <class T> struct Unit {
+    T v[UV<T>];
+    static __device__ __forceinline__ Unit load(const T* p, int n) {
+        Unit u;
+        if (n >= UV<T>) {
+            const typename Raw<T>::type r = *(const typename Raw<T>::type*)p;
+            __builtin_memcpy(u.v, &r, 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < UV<T>; j++) u.v[j] = j < n ? p[j] : T(0.0f);
+        }
+        return u;
+    }
+    __device__ __forceinline__ void store(T* p, int n) const {
+        if (n >= UV<T>) {
+            typename Raw<T>::type r;
+            __builtin_memcpy(&r, v, 16);
+            *(typename Raw<T>::type*)p = r;
+        } else {
+#pragma unroll
+            for (int j = 0; j < UV<T>; j++) if (j < n) p[j] = v[j];
+        }
+    }
+};
+
+// How a grid of blocks walks rows of `upr` units each, one unit per lane: short rows share a block (`rpb` rows of them), a long row is cut
+// into `segs` segments (rpb = 0).  The block size is the multiple of a wave that leaves the fewest lanes without a unit.  The quotient
+// i / upr of a unit's index in its block is exact for i, upr < 2^16.
+struct Walk {
+    int64_t rows, upr, segs, blocks;
+    int32_t rpb, block;
+    uint32_t magic;
+};
+inline Walk walk_of(size_t rows, size_t upr) {
+    Walk w{(int64_t)rows, (int64_t)upr, 0, 0, 0, 256, 0};
+    double best = 0;
+    for (int block : {256, 192, 320, 384, 128, 448, 512, 64}) {
+        const size_t b = (size_t)block, used = upr <= b ? b / upr * upr : upr, of = upr <= b ? b : (upr + b - 1) / b * b;
+        const double share = (double)used / (double)of;
+        if (share > best + 0.01) { best = share; w.block = block; }
+    }
+    const size_t b = (size_t)w.block;
+    if (upr <= b) {
+        w.rpb = (int32_t)(b / upr);
+        w.magic = (uint32_t)(((uint64_t)1 << 32) / upr + 1);
+        w.blocks = (int64_t)((rows + w.rpb - 1) / w.rpb);
+    } else {
+        w.segs = (int64_t)((upr + b - 1) / b);
+        w.blocks = (int64_t)rows * w.segs;
+    }
+    return w;
+}
+GL_DEV bool walk_unit(const Walk& w, int64_t* r, int64_t* u) {   // this lane's unit; false: there is none
+    const int i = (int)threadIdx.x;
+    if (w.rpb) {
+        const uint32_t q = w.upr == 1 ? (uint32_t)i : (uint32_t)(((uint64_t)(uint32_t)i * w.magic) >> 32);
+        *r = (int64_t)blockIdx.x * w.rpb + q;
+        *u = i - (int64_t)q * w.upr;
+        return (int)q < w.rpb && *r < w.rows;
+    }
+    const int64_t b = (int64_t)blockIdx.x / w.segs;
+    *r = b;
+    *u = ((int64_t)blockIdx.x - b * w.segs) * w.block + i;
+    return *u < w.upr;
 }
 
 struct Slots {   // where frame r goes / comes from
@@ -74,8 +148,9 @@ struct WriteArgs {
     Slots slots;
     uint8_t* store;
     CacheLayout l;
-    const int32_t* claim;
+    int32_t* claim;           // null: a frame looks through the later slots of the call itself
     unsigned long long* bad;
+    int32_t lanes_log2, gunits_log2, segs;
 };
 struct ReadArgs {
     void* y;
@@ -83,14 +158,16 @@ struct ReadArgs {
     Slots slots;
     const uint8_t* store;
     CacheLayout l;
+    Walk w;
     DropRule drop;
-    int32_t dropping, strict;
+    int32_t gshift, strict;   // a band's group = band >> gshift
     uint64_t seed, offset;
     unsigned long long* bad;
 };
 
 // Which frame keeps a slot that a write names more than once: the last.  The rows of a call claim their slots with an atomic maximum
-// of the row index, the write below keeps the row whose claim stands, and k_claim_clear puts the -1 back.
+// of the row index, the write below keeps the row whose claim stands and puts the -1 back (k_claim_clear does where several parts of the
+// grid share a frame).
 __global__ void k_claim(Slots s, int64_t n, int32_t* claim) {
     const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (r >= n) return;
@@ -104,98 +181,299 @@ __global__ void k_claim_clear(Slots s, int64_t n, int32_t* claim) {
     if (slot >= 0 && slot < s.n_slots) claim[slot] = -1;
 }
 
-// One wave per frame, group after group: extremes, then codes (the second reading of the group comes from the cache).
-template <class T> __global__ __launch_bounds__(64) void k_write(WriteArgs a) {
+// Extremes of a group while they are being gathered: `odd` turns NaN once a value is not finite.
+template <class W> struct Range {
+    W mn = (W)__builtin_inf(), mx = -(W)__builtin_inf(), odd = 0;
+    __device__ __forceinline__ void add(float v) { mn = fminf(mn, v); mx = fmaxf(mx, v); odd = fmaf(v, 0.0f, odd); }
+    __device__ __forceinline__ void add(double v) { mn = fmin(mn, v); mx = fmax(mx, v); odd = fma(v, 0.0, odd); }
+};
+GL_DEV float least(float a, float b) { return fminf(a, b); }
+GL_DEV double least(double a, double b) { return fmin(a, b); }
+GL_DEV float most(float a, float b) { return fmaxf(a, b); }
+GL_DEV double most(double a, double b) { return fmax(a, b); }
+// The same with the finite values only, and what the others are (group_scale's flags).
+template <class W> GL_DEV void add_finite(W v, W* mn, W* mx, int* flags) {
+    if (v != v) *flags |= 1;
+    else if (v == (W)__builtin_inf()) *flags |= 2;
+    else if (v == -(W)__builtin_inf()) *flags |= 4;
+    else { *mn = least(*mn, v); *mx = most(*mx, v); }
+}
+GL_DEV double reciprocal(Scale s) { return s.step > 0.0f ? 1.0 / (double)s.step : 0.0; }
+
+// One unit's codes into the row and, when they are asked for, its values.
+template <class T> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row, T* y, bool keep, int u, int n, const typename Wide<T>::type* w, Scale s, double per) {
     typedef typename Wide<T>::type W;
-    const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x, K = a.l.K, levels = (1 << a.l.bits) - 1;
-    const int64_t slot = slot_of(a.slots, r);
-    if (slot < 0 || slot >= a.slots.n_slots) {
-        if (slot >= a.slots.n_slots && lane == 0) atomicAdd(a.bad, 1ull);
-        return;
+    const bool wide = a.l.bits == 8;
+    const float levels = wide ? 255.0f : 15.0f;
+    Unit<T> out;
+    uint32_t code[2] = {0, 0};
+    float q[UV<T>];
+#pragma unroll
+    for (int j = 0; j < UV<T>; j++) q[j] = quantise((double)w[j], s, per, levels);
+    if (keep) {
+        if (wide) {
+#pragma unroll
+            for (int j = 0; j < UV<T>; j++) code[j / 4] |= (uint32_t)q[j] << (8 * (j % 4));
+            __builtin_memcpy(__builtin_assume_aligned(row + u * UV<T>, UV<T>), code, UV<T>);
+        } else {
+#pragma unroll
+            for (int j = 0; j < UV<T>; j++) code[0] |= (uint32_t)q[j] << (4 * j);
+            __builtin_memcpy(__builtin_assume_aligned(row + u * (UV<T> / 2), UV<T> / 2), code, UV<T> / 2);
+        }
     }
-    const bool keep = !a.claim || a.claim[slot] == (int32_t)r;
-    const T* x = (const T*)a.x + r * a.xs;
-    T* y = a.y ? (T*)a.y + r * a.ys : nullptr;
-    uint8_t* row = a.store + slot * a.l.row_bytes;
-    for (int g = 0; g < a.l.groups; g++) {
-        const int b0 = g * a.l.group, b1 = min(K, b0 + a.l.group);
-        double mn = __builtin_inf(), mx = -__builtin_inf();
-        int flags = 0;
-        for (int i = 2 * b0 + lane; i < 2 * b1; i += 64) {
-            const double v = (double)widen(x[i]);
-            if (v != v) flags |= 1;
-            else if (v == __builtin_inf()) flags |= 2;
-            else if (v == -__builtin_inf()) flags |= 4;
-            else { mn = fmin(mn, v); mx = fmax(mx, v); }
-        }
-        for (int m = 1; m < 64; m <<= 1) {
-            mn = fmin(mn, __shfl_xor(mn, m));
-            mx = fmax(mx, __shfl_xor(mx, m));
-            flags |= __shfl_xor(flags, m);
-        }
-        const Scale s = group_scale(mn, mx, flags, levels);
-        if (keep && lane == 0) *(float2*)(row + a.l.scale_off + 8 * g) = make_float2(s.lo, s.step);
-        for (int b = b0 + lane; b < b1; b += 64) {
-            const int q0 = quantise((double)widen(x[2 * b]), s, levels), q1 = quantise((double)widen(x[2 * b + 1]), s, levels);
-            if (keep) {
-                if (a.l.bits == 8) { row[2 * b] = (uint8_t)q0; row[2 * b + 1] = (uint8_t)q1; }
-                else row[b] = (uint8_t)(q0 | q1 << 4);
-            }
-            if (y) { y[2 * b] = narrow<T>(dequantise(q0, s, W(0))); y[2 * b + 1] = narrow<T>(dequantise(q1, s, W(0))); }
-        }
+    if (y) {
+#pragma unroll
+        for (int j = 0; j < UV<T>; j++) out.v[j] = narrow<T>(dequantise(q[j], s, W(0)));
+        out.store(y + (int64_t)u * UV<T>, n);
     }
 }
 
-// One lane per band.
-template <class T> __global__ __launch_bounds__(64) void k_read(ReadArgs a) {
+// A frame -- or, of a wide grouped one, a segment of it -- lies in the registers of 2^lanes_log2 neighbouring lanes, NC units each, `lanes`
+// apart, so that every load of the wave is one run of memory.  Its extremes are joined across those lanes (a group's across the lanes
+// of the group), the codes follow from the same registers: the frames are read once.
+template <class T, int NC, bool GROUPED> __global__ __launch_bounds__(256) void k_write(WriteArgs a) {
     typedef typename Wide<T>::type W;
-    const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x;
+    const int lanes = 1 << a.lanes_log2, l = (int)threadIdx.x & (lanes - 1);
+    const int64_t part = (int64_t)blockIdx.x * (256 >> a.lanes_log2) + ((int)threadIdx.x >> a.lanes_log2);
+    if (part >= a.n * a.segs) return;
+    const int64_t r = a.segs == 1 ? part : part / a.segs;
+    const int u0 = a.segs == 1 ? 0 : (int)(part - r * a.segs) * (NC * lanes);
+    const T* x = (const T*)a.x + r * a.xs;
+    Unit<T> in[NC];
+    int n[NC];
+#pragma unroll
+    for (int k = 0; k < NC; k++) {
+        const int c = (u0 + l + k * lanes) * UV<T>;
+        n[k] = min(UV<T>, 2 * a.l.K - c);
+        if (n[k] > 0) in[k] = Unit<T>::load(x + c, n[k]);
+    }
     const int64_t slot = slot_of(a.slots, r);
     if (slot < 0 || slot >= a.slots.n_slots) {
-        if ((slot >= a.slots.n_slots || a.strict) && lane == 0) atomicAdd(a.bad, 1ull);
+        if (slot >= a.slots.n_slots && l == 0 && u0 == 0) atomicAdd(a.bad, 1ull);
+        return;
+    }
+    const int first = (int)(threadIdx.x & 63) & ~(lanes - 1);   // of this frame's lanes in the wave
+    bool keep = true;
+    if (a.claim) {
+        keep = a.claim[slot] == (int32_t)r;
+        if (keep && l == 0 && a.segs == 1) a.claim[slot] = -1;   // (a frame that lost reads its rival's index or this: neither is its own)
+    } else if (a.slots.at && a.n > 1) {
+        bool again = false;
+        for (int64_t i = r + 1 + l; i < a.n; i += lanes) again |= a.slots.at[i] == slot;
+        keep = !(__ballot(again) >> first & (~0ull >> (64 - lanes)));
+    }
+    uint8_t* row = a.store + slot * a.l.row_bytes;
+    T* y = a.y ? (T*)a.y + r * a.ys : nullptr;
+    W w[NC][UV<T>];
+    Range<W> range[GROUPED ? NC : 1];
+#pragma unroll
+    for (int k = 0; k < NC; k++)
+#pragma unroll
+        for (int j = 0; j < UV<T>; j++) {
+            w[k][j] = j < n[k] ? widen(in[k].v[j]) : W(0);
+            if (j < n[k]) range[GROUPED ? k : 0].add(w[k][j]);
+        }
+    const int span = GROUPED ? 1 << a.gunits_log2 : lanes;          // lanes that hold a group
+    const int start = (int)(threadIdx.x & 63) & ~(span - 1);
+    const int levels = (1 << a.l.bits) - 1;
+#pragma unroll
+    for (int g = 0; g < (GROUPED ? NC : 1); g++) {
+        W mn = range[g].mn, mx = range[g].mx;
+        for (int m = 1; m < span; m <<= 1) { mn = least(mn, __shfl_xor(mn, m)); mx = most(mx, __shfl_xor(mx, m)); }
+        int flags = 0;
+        if (__ballot(!(range[g].odd == W(0))) >> start & (~0ull >> (64 - span))) {
+            mn = (W)__builtin_inf(); mx = -(W)__builtin_inf();
+#pragma unroll
+            for (int k = GROUPED ? g : 0; k < (GROUPED ? g + 1 : NC); k++)
+#pragma unroll
+                for (int j = 0; j < UV<T>; j++) if (j < n[k]) add_finite(w[k][j], &mn, &mx, &flags);
+            for (int m = 1; m < span; m <<= 1) { mn = least(mn, __shfl_xor(mn, m)); mx = most(mx, __shfl_xor(mx, m)); flags |= __shfl_xor(flags, m); }
+        }
+        const Scale s = group_scale((double)mn, (double)mx, flags, levels);
+        const double per = reciprocal(s);
+        const int ug = u0 + l + g * lanes;                          // GROUPED: the unit whose group this is
+        if (keep && (GROUPED ? ((ug & (span - 1)) == 0 && n[g] > 0) : l == 0))
+            *(float2*)(row + a.l.scale_off + 8 * (GROUPED ? ug >> a.gunits_log2 : 0)) = make_float2(s.lo, s.step);
+#pragma unroll
+        for (int k = GROUPED ? g : 0; k < (GROUPED ? g + 1 : NC); k++)
+            if (n[k] > 0) put_unit<T>(a, row, y, keep, u0 + l + k * lanes, n[k], w[k], s, per);
+    }
+}
+
+// A frame under one scale that is too wide for a wave's registers: a block per frame, which reads it twice (the second time out of the
+// caches: at most 256 KB).
+template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs a) {
+    typedef typename Wide<T>::type W;
+    __shared__ W s_mn[4], s_mx[4];
+    __shared__ int s_flags[4];
+    const int64_t r = blockIdx.x, slot = slot_of(a.slots, r);
+    const int t = (int)threadIdx.x, cols = 2 * a.l.K;
+    if (slot < 0 || slot >= a.slots.n_slots) {
+        if (slot >= a.slots.n_slots && t == 0) atomicAdd(a.bad, 1ull);
+        return;
+    }
+    bool keep = true;
+    if (a.claim) {
+        keep = a.claim[slot] == (int32_t)r;
+        __syncthreads();
+        if (keep && t == 0) a.claim[slot] = -1;
+    } else if (a.slots.at && a.n > 1) {
+        int again = 0;
+        for (int64_t i = r + 1 + t; i < a.n; i += 256) again |= a.slots.at[i] == slot;
+        keep = !__syncthreads_or(again);
+    }
+    const T* x = (const T*)a.x + r * a.xs;
+    W mn = (W)__builtin_inf(), mx = -(W)__builtin_inf();
+    int flags = 0;
+    for (int c = t * UV<T>; c < cols; c += 256 * UV<T>) {
+        const int n = min(UV<T>, cols - c);
+        const Unit<T> in = Unit<T>::load(x + c, n);
+#pragma unroll
+        for (int j = 0; j < UV<T>; j++) if (j < n) add_finite(widen(in.v[j]), &mn, &mx, &flags);
+    }
+    for (int m = 1; m < 64; m <<= 1) { mn = least(mn, __shfl_xor(mn, m)); mx = most(mx, __shfl_xor(mx, m)); flags |= __shfl_xor(flags, m); }
+    if ((t & 63) == 0) { s_mn[t >> 6] = mn; s_mx[t >> 6] = mx; s_flags[t >> 6] = flags; }
+    __syncthreads();
+    for (int i = 0; i < 4; i++) { mn = least(mn, s_mn[i]); mx = most(mx, s_mx[i]); flags |= s_flags[i]; }
+    const Scale s = group_scale((double)mn, (double)mx, flags, (1 << a.l.bits) - 1);
+    const double per = reciprocal(s);
+    uint8_t* row = a.store + slot * a.l.row_bytes;
+    T* y = a.y ? (T*)a.y + r * a.ys : nullptr;
+    if (keep && t == 0) *(float2*)(row + a.l.scale_off) = make_float2(s.lo, s.step);
+    for (int c = t * UV<T>; c < cols; c += 256 * UV<T>) {
+        const int n = min(UV<T>, cols - c);
+        const Unit<T> in = Unit<T>::load(x + c, n);
+        W w[UV<T>];
+#pragma unroll
+        for (int j = 0; j < UV<T>; j++) w[j] = j < n ? widen(in.v[j]) : W(0);
+        put_unit<T>(a, row, y, keep, c / UV<T>, n, w, s, per);
+    }
+}
+
+// The 32 random bits of the N elements from `e` on: one word of the generator for two elements, its argument stepped from word to word;
+// an odd start straddles words and needs one more.  The word's index has 63 bits, so where the element's 64 wrap to zero the step
+// would be wrong: elements that may be there take their words one by one.
+template <int N> GL_DEV void random_bits(uint64_t seed, uint64_t e, uint32_t* u) {
+    const uint64_t i = e >> 1;
+    uint64_t z = seed + (i + 1) * kGamma;
+    if ((uint32_t)(i >> 32) == 0x7FFFFFFFu) {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const uint64_t at = e + (uint32_t)j, w = splitmix_of(seed + ((at >> 1) + 1) * kGamma);
+            u[j] = (uint32_t)((at & 1) ? w >> 32 : w);
+        }
+    } else if (!(e & 1)) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2, z += kGamma) {
+            const uint64_t w = splitmix_of(z);
+            u[j] = (uint32_t)w;
+            u[j + 1] = (uint32_t)(w >> 32);
+        }
+    } else {
+        uint32_t before = (uint32_t)(splitmix_of(z) >> 32);
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            z += kGamma;
+            const uint64_t w = splitmix_of(z);
+            u[j] = before;
+            u[j + 1] = (uint32_t)w;
+            before = (uint32_t)(w >> 32);
+        }
+    }
+}
+template <class T> GL_DEV void drop_unit(Unit<T>* x, const DropRule& d, const uint32_t* u) {
+    typedef typename Wide<T>::type W;
+#pragma unroll
+    for (int j = 0; j < UV<T>; j++) x->v[j] = narrow<T>(((uint32_t)d.all | (uint32_t)(u[j] < d.below)) ? W(0) : widen(x->v[j]) * (W)d.scale);
+}
+
+// One unit of the output per lane: its codes (2 ... 8 bytes), its group's scale, one 16-byte store.  Bound by HBM, most of it the output's
+// writing.
+template <class T, int BITS, bool DROP> __global__ __launch_bounds__(512) void k_read(ReadArgs a) {
+    typedef typename Wide<T>::type W;
+    int64_t r, u64;
+    if (!walk_unit(a.w, &r, &u64)) return;
+    const int u = (int)u64, c = u * UV<T>, n = min(UV<T>, 2 * a.l.K - c);
+    const int64_t slot = slot_of(a.slots, r);
+    if (slot < 0 || slot >= a.slots.n_slots) {
+        if ((slot >= a.slots.n_slots || a.strict) && u == 0) atomicAdd(a.bad, 1ull);
         return;
     }
     const uint8_t* row = a.store + slot * a.l.row_bytes;
-    T* y = (T*)a.y + r * a.ys;
-    for (int b = lane; b < a.l.K; b += 64) {
-        const float2 f = *(const float2*)(row + a.l.scale_off + 8 * (b / a.l.group));
-        const Scale s{f.x, f.y};
-        const int q0 = a.l.bits == 8 ? row[2 * b] : row[b] & 15, q1 = a.l.bits == 8 ? row[2 * b + 1] : row[b] >> 4;
-        W v0 = dequantise(q0, s, W(0)), v1 = dequantise(q1, s, W(0));
-        if (a.dropping) {
-            const uint64_t e = a.offset + (uint64_t)r * (2 * a.l.K) + 2 * b;
-            v0 = dropped(a.drop, a.seed, e) ? W(0) : v0 * (W)a.drop.scale;
-            v1 = dropped(a.drop, a.seed, e + 1) ? W(0) : v1 * (W)a.drop.scale;
-        }
-        y[2 * b] = narrow<T>(v0); y[2 * b + 1] = narrow<T>(v1);
+    constexpr int CB = UV<T> * BITS / 8;   // a row's codes are padded to 16 bytes: a partial unit's are there too
+    uint32_t code[CB > 4 ? 2 : 1];
+    code[0] = 0;
+    __builtin_memcpy(code, __builtin_assume_aligned(row + (int64_t)u * CB, CB), CB);
+    const float2 f = *(const float2*)(row + a.l.scale_off + 8 * ((c >> 1) >> a.gshift));
+    const Scale s{f.x, f.y};
+    uint32_t bits[UV<T>];
+    if (DROP) {
+        const uint64_t e = a.offset + (uint64_t)r * (uint32_t)(2 * a.l.K) + (uint32_t)c;
+        random_bits<UV<T>>(a.seed, e, bits);
     }
+    Unit<T> out;
+#pragma unroll
+    for (int j = 0; j < UV<T>; j++) {
+        const uint32_t q = code[j * BITS / 32] >> (j * BITS % 32) & ((1u << BITS) - 1);
+        W v = dequantise((float)q, s, W(0));
+        if (DROP) v = ((uint32_t)a.drop.all | (uint32_t)(bits[j] < a.drop.below)) ? W(0) : v * (W)a.drop.scale;
+        out.v[j] = narrow<T>(v);
+    }
+    out.store((T*)a.y + r * a.ys + c, n);
 }
 
 struct DropArgs {
     const void* x; void* y;
-    int64_t xs, ys, rows, cols;
+    int64_t xs, ys, cols, total;
+    Walk w;
     DropRule drop;
     uint64_t seed, offset;
 };
+// Dense arrays: one unit per lane.  Bound by HBM in fp32 and fp64 (two streams), by the generator's multiplications in the 16-bit types:
+// six quarter-rate 32-bit products for two elements.  One unit per lane is the best of 1, 2, 4 and 8: with more in flight per lane
+// fp32 falls from 6.17 to 5.9 TB/s, bf16 from 6.08 to 5.8 (409 600 x 384 elements, bytes read and written).
 template <class T> __global__ __launch_bounds__(256) void k_dropout(DropArgs a) {
-    typedef typename Wide<T>::type W;
-    const int64_t total = a.rows * a.cols;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / a.cols, k = i - r * a.cols;
-        const W v = widen(((const T*)a.x)[r * a.xs + k]);
-        ((T*)a.y)[r * a.ys + k] = narrow<T>(dropped(a.drop, a.seed, a.offset + (uint64_t)i) ? W(0) : v * (W)a.drop.scale);
-    }
+    const int64_t e0 = (int64_t)blockIdx.x * (256 * UV<T>);
+    const int t = (int)threadIdx.x * UV<T>;
+    const int n = (int)min((int64_t)UV<T>, a.total - e0 - t);
+    if (n <= 0) return;
+    Unit<T> x = Unit<T>::load((const T*)a.x + e0 + t, n);
+    uint32_t u[UV<T>];
+    random_bits<UV<T>>(a.seed, a.offset + (uint64_t)e0 + (uint32_t)t, u);
+    drop_unit(&x, a.drop, u);
+    x.store((T*)a.y + e0 + t, n);
+}
+// Rows apart.
+template <class T> __global__ __launch_bounds__(512) void k_dropout_rows(DropArgs a) {
+    int64_t r, k;
+    if (!walk_unit(a.w, &r, &k)) return;
+    const int64_t c = k * UV<T>;
+    const int n = (int)min((int64_t)UV<T>, a.cols - c);
+    Unit<T> x = Unit<T>::load((const T*)a.x + r * a.xs + c, n);
+    const uint64_t e = a.offset + (uint64_t)(r * a.cols + c);
+    uint32_t u[UV<T>];
+    random_bits<UV<T>>(a.seed, e, u);
+    drop_unit(&x, a.drop, u);
+    x.store((T*)a.y + r * a.ys + c, n);
 }
 
-#define GL_TYPES(type, CALL)                                  \
-    switch (type) {                                           \
-        case GOMEL_F64: { typedef double T; CALL; } break;    \
-        case GOMEL_F32: { typedef float T; CALL; } break;     \
-        case GOMEL_F16: { typedef __half T; CALL; } break;    \
-        default: { typedef __hip_bfloat16 T; CALL; } break;   \
+#define GL_TYPES(type, ...)                                          \
+    switch (type) {                                                  \
+        case GOMEL_F64: { typedef double T; __VA_ARGS__; } break;    \
+        case GOMEL_F32: { typedef float T; __VA_ARGS__; } break;     \
+        case GOMEL_F16: { typedef __half T; __VA_ARGS__; } break;    \
+        default: { typedef __hip_bfloat16 T; __VA_ARGS__; } break;   \
     }
+template <class T> void (*write_kernel(int units, bool grouped))(WriteArgs) {
+    switch (units) {
+        case 1: return grouped ? k_write<T, 1, true> : k_write<T, 1, false>;
+        case 2: return grouped ? k_write<T, 2, true> : k_write<T, 2, false>;
+        case 3: return grouped ? k_write<T, 3, true> : k_write<T, 3, false>;
+        case 4: return grouped ? k_write<T, 4, true> : k_write<T, 4, false>;
+        case 5: return grouped ? k_write<T, 5, true> : k_write<T, 5, false>;
+        default: return grouped ? k_write<T, 6, true> : k_write<T, 6, false>;
+    }
+}
 // launches report their own status: hipGetLastError could hand back somebody else's
 template <class Args> hipError_t launch(void (*k)(Args), unsigned grid, unsigned block, hipStream_t s, Args& a) {
     void* p[] = {&a};
@@ -227,14 +505,24 @@ bool capturing(hipStream_t s) {
 }
 
 hipError_t dropout_device(int type, const void* x, size_t xs, void* y, size_t ys, size_t rows, size_t cols, const DropRule& d, uint64_t seed, uint64_t offset, hipStream_t s) {
-    DropArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)rows, (int64_t)cols, d, seed, offset};
-    const unsigned grid = (unsigned)std::min<size_t>((rows * cols + 255) / 256, 65536);
+    const size_t total = rows * cols, uv = 16 / (size_t)type_bytes(type);
+    DropArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)cols, (int64_t)total, Walk{}, d, seed, offset};
     hipError_t e = hipSuccess;
-    GL_TYPES(type, e = launch(k_dropout<T>, grid, 256, s, a));
+    if ((xs == cols && ys == cols) || rows == 1) {
+        const size_t units = (total + uv - 1) / uv, blocks = (units + 256 - 1) / 256;
+        if (blocks > INT32_MAX) return hipErrorInvalidValue;
+        GL_TYPES(type, e = launch(k_dropout<T>, (unsigned)blocks, 256, s, a));
+        return e;
+    }
+    a.w = walk_of(rows, (cols + uv - 1) / uv);
+    if (a.w.blocks > INT32_MAX) return hipErrorInvalidValue;
+    GL_TYPES(type, e = launch(k_dropout_rows<T>, (unsigned)a.w.blocks, (unsigned)a.w.block, s, a));
     return e;
 }
 
 constexpr size_t kStageBytes = (size_t)32 << 20;
+constexpr size_t kScanRows = 2048;   // frames of a write up to which each looks through the later slots itself; more claim theirs first
+constexpr int kMostUnits = 6;        // units a lane of k_write holds
 
 // Rows between host memory (stride elements apart) and a dense device buffer
 hipError_t rows_in(void* dev, const char* host, size_t stride, size_t rows, size_t cols, size_t esz, hipStream_t s) {
@@ -387,21 +675,47 @@ int memory_kind(const void* p, int device) {
 }
 
 hipError_t cache_write_device(gomel_cache* c, int type, const void* x, size_t xs, size_t n, const int64_t* slots, size_t first, void* y, size_t ys, hipStream_t s) {
-    const bool claims = slots && n > 1;
-    WriteArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, claims ? c->claim : nullptr, c->bad};
+    const bool claims = slots && n > kScanRows;
+    WriteArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, claims ? c->claim : nullptr, c->bad, 6, 0, 1};
+    const int uv = 16 / type_bytes(type), upr = (2 * c->l.K + uv - 1) / uv;
+    const bool grouped = c->l.groups > 1;
+    int least_lanes = 3, nc = 0;
+    if (grouped) {
+        while ((uv << a.gunits_log2) < 2 * c->l.group) a.gunits_log2++;
+        least_lanes = std::max(least_lanes, a.gunits_log2);
+    }
+    // lanes x units per lane: the pair with the fewest idle places, the most lanes among equals
+    for (int lg = 6, best = INT32_MAX; lg >= least_lanes; lg--) {
+        const int k = (upr + (1 << lg) - 1) >> lg;
+        if (k <= kMostUnits && (k << lg) < best) { best = k << lg; nc = k; a.lanes_log2 = lg; }
+    }
     hipError_t e = hipSuccess;
     if (claims) e = launch_claim(k_claim, a.slots, a.n, c->claim, s);
-    if (e == hipSuccess) GL_TYPES(type, e = launch(k_write<T>, (unsigned)n, 64, s, a));
-    if (claims && e == hipSuccess) e = launch_claim(k_claim_clear, a.slots, a.n, c->claim, s);
+    if (e != hipSuccess) return e;
+    if (!nc && !grouped) {
+        GL_TYPES(type, e = launch(k_write_wide<T>, (unsigned)n, 256, s, a));
+        return e;
+    }
+    if (!nc) { nc = 4; a.segs = (upr + 255) / 256; }   // wide and grouped: segments of 64 lanes x 4 units, whole groups each
+    const size_t per = 256 >> a.lanes_log2, blocks = (n * (size_t)a.segs + per - 1) / per;
+    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    GL_TYPES(type, e = launch(write_kernel<T>(nc, grouped), (unsigned)blocks, 256, s, a));
+    if (claims && a.segs > 1 && e == hipSuccess) e = launch_claim(k_claim_clear, a.slots, a.n, c->claim, s);
     return e;
 }
 
 hipError_t cache_read_device(gomel_cache* c, int type, void* y, size_t ys, size_t n, const int64_t* slots, size_t first, const DropRule& drop,
                              uint64_t seed, uint64_t offset, bool strict, unsigned long long* bad, hipStream_t s) {
-    ReadArgs a{y, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, drop, (int32_t)(drop.all || drop.below != 0),
-               (int32_t)strict, seed, offset, bad ? bad : c->bad};
+    const int uv = 16 / type_bytes(type);
+    int gshift = 31;
+    if (c->l.groups > 1) for (gshift = 0; (1 << gshift) < c->l.group; gshift++) {}
+    ReadArgs a{y, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, walk_of(n, (size_t)(2 * c->l.K + uv - 1) / uv), drop,
+               gshift, (int32_t)strict, seed, offset, bad ? bad : c->bad};
+    if (a.w.blocks > INT32_MAX) return hipErrorInvalidValue;
+    const bool wide = c->l.bits == 8, dropping = drop.all || drop.below != 0;
     hipError_t e = hipSuccess;
-    GL_TYPES(type, e = launch(k_read<T>, (unsigned)n, 64, s, a));
+    GL_TYPES(type, e = launch(dropping ? (wide ? k_read<T, 8, true> : k_read<T, 4, true>) : (wide ? k_read<T, 8, false> : k_read<T, 4, false>),
+                              (unsigned)a.w.blocks, (unsigned)a.w.block, s, a));
     return e;
 }
 
