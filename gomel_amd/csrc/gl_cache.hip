@@ -72,10 +72,12 @@ template <> struct Raw<__half> { typedef raw_any type; };
 template <> struct Raw<__hip_bfloat16> { typedef raw_any type; };
 template <class T> struct Unit {
     T v[UV<T>];
-    static __device__ __forceinline__ Unit load(const T* p, int n) {
+    template <bool S> static __device__ __forceinline__ Unit load(const T* p, int n) {
         Unit u;
         if (n >= UV<T>) {
-            const typename Raw<T>::type r = *(const typename Raw<T>::type*)p;
+            typename Raw<T>::type r;
+            if (S) r = __builtin_nontemporal_load((const typename Raw<T>::type*)p);
+            else r = *(const typename Raw<T>::type*)p;
             __builtin_memcpy(u.v, &r, 16);
         } else {
 #pragma unroll
@@ -83,17 +85,34 @@ template <class T> struct Unit {
         }
         return u;
     }
-    __device__ __forceinline__ void store(T* p, int n) const {
+    template <bool S> __device__ __forceinline__ void store(T* p, int n) const {
         if (n >= UV<T>) {
             typename Raw<T>::type r;
             __builtin_memcpy(&r, v, 16);
-            *(typename Raw<T>::type*)p = r;
+            if (S) __builtin_nontemporal_store(r, (typename Raw<T>::type*)p);
+            else *(typename Raw<T>::type*)p = r;
         } else {
 #pragma unroll
             for (int j = 0; j < UV<T>; j++) if (j < n) p[j] = v[j];
         }
     }
 };
+
+// How a frame lies over a wave: in 2^lanes_log2 neighbouring lanes, `units` units each, `lanes` apart, so that every access of the wave is
+// one run of memory and what depends on the frame alone (its slot, its addresses) is worked out once per lane.  A frame too wide for
+// that is cut into `segs` segments of 64 lanes x 4 units (units = 0: k_write cannot, it needs the extremes of the whole frame).
+struct Spread { int32_t lanes_log2, units, segs; };
+constexpr int kMostUnits = 6;
+inline Spread spread_of(int upr, int least_lanes_log2, bool may_cut) {
+    Spread p{6, 0, 1};
+    // the pair with the fewest idle places, the most lanes among equals
+    for (int lg = 6, best = INT32_MAX; lg >= least_lanes_log2; lg--) {
+        const int k = (upr + (1 << lg) - 1) >> lg;
+        if (k <= kMostUnits && (k << lg) < best) { best = k << lg; p.units = k; p.lanes_log2 = lg; }
+    }
+    if (!p.units && may_cut) { p.units = 4; p.segs = (upr + 255) / 256; }
+    return p;
+}
 
 // How a grid of blocks walks rows of `upr` units each, one unit per lane: short rows share a block (`rpb` rows of them), a long row is cut
 // into `segs` segments (rpb = 0).  The block size is the multiple of a wave that leaves the fewest lanes without a unit.  The quotient
@@ -150,7 +169,8 @@ struct WriteArgs {
     CacheLayout l;
     int32_t* claim;           // null: a frame looks through the later slots of the call itself
     unsigned long long* bad;
-    int32_t lanes_log2, gunits_log2, segs;
+    Spread p;
+    int32_t gunits_log2;      // a group's units
 };
 struct ReadArgs {
     void* y;
@@ -158,11 +178,12 @@ struct ReadArgs {
     Slots slots;
     const uint8_t* store;
     CacheLayout l;
-    Walk w;
+    Spread p;
     DropRule drop;
     int32_t gshift, strict;   // a band's group = band >> gshift
     uint64_t seed, offset;
     unsigned long long* bad;
+    int32_t wraps;            // offset + the output's elements pass 2^64
 };
 
 // Which frame keeps a slot that a write names more than once: the last.  The rows of a call claim their slots with an atomic maximum
@@ -201,7 +222,7 @@ template <class W> GL_DEV void add_finite(W v, W* mn, W* mx, int* flags) {
 GL_DEV double reciprocal(Scale s) { return s.step > 0.0f ? 1.0 / (double)s.step : 0.0; }
 
 // One unit's codes into the row and, when they are asked for, its values.
-template <class T> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row, T* y, bool keep, int u, int n, const typename Wide<T>::type* w, Scale s, double per) {
+template <class T, bool S> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row, T* y, bool keep, int u, int n, const typename Wide<T>::type* w, Scale s, double per) {
     typedef typename Wide<T>::type W;
     const bool wide = a.l.bits == 8;
     const float levels = wide ? 255.0f : 15.0f;
@@ -224,20 +245,19 @@ template <class T> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row, T* y, 
     if (y) {
 #pragma unroll
         for (int j = 0; j < UV<T>; j++) out.v[j] = narrow<T>(dequantise(q[j], s, W(0)));
-        out.store(y + (int64_t)u * UV<T>, n);
+        out.template store<S>(y + (int64_t)u * UV<T>, n);
     }
 }
 
-// A frame -- or, of a wide grouped one, a segment of it -- lies in the registers of 2^lanes_log2 neighbouring lanes, NC units each, `lanes`
-// apart, so that every load of the wave is one run of memory.  Its extremes are joined across those lanes (a group's across the lanes
-// of the group), the codes follow from the same registers: the frames are read once.
-template <class T, int NC, bool GROUPED> __global__ __launch_bounds__(256) void k_write(WriteArgs a) {
+// A frame -- or, of a wide grouped one, a segment of it -- lies in the registers of its lanes (Spread).  Its extremes are joined across
+// those lanes (a group's across the lanes of the group), the codes follow from the same registers: the frames are read once.
+template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(256) void k_write(WriteArgs a) {
     typedef typename Wide<T>::type W;
-    const int lanes = 1 << a.lanes_log2, l = (int)threadIdx.x & (lanes - 1);
-    const int64_t part = (int64_t)blockIdx.x * (256 >> a.lanes_log2) + ((int)threadIdx.x >> a.lanes_log2);
-    if (part >= a.n * a.segs) return;
-    const int64_t r = a.segs == 1 ? part : part / a.segs;
-    const int u0 = a.segs == 1 ? 0 : (int)(part - r * a.segs) * (NC * lanes);
+    const int lanes = 1 << a.p.lanes_log2, l = (int)threadIdx.x & (lanes - 1);
+    const int64_t part = (int64_t)blockIdx.x * (256 >> a.p.lanes_log2) + ((int)threadIdx.x >> a.p.lanes_log2);
+    if (part >= a.n * a.p.segs) return;
+    const int64_t r = a.p.segs == 1 ? part : part / a.p.segs;
+    const int u0 = a.p.segs == 1 ? 0 : (int)(part - r * a.p.segs) * (NC * lanes);
     const T* x = (const T*)a.x + r * a.xs;
     Unit<T> in[NC];
     int n[NC];
@@ -245,7 +265,7 @@ template <class T, int NC, bool GROUPED> __global__ __launch_bounds__(256) void 
     for (int k = 0; k < NC; k++) {
         const int c = (u0 + l + k * lanes) * UV<T>;
         n[k] = min(UV<T>, 2 * a.l.K - c);
-        if (n[k] > 0) in[k] = Unit<T>::load(x + c, n[k]);
+        if (n[k] > 0) in[k] = Unit<T>::template load<S>(x + c, n[k]);
     }
     const int64_t slot = slot_of(a.slots, r);
     if (slot < 0 || slot >= a.slots.n_slots) {
@@ -256,7 +276,7 @@ template <class T, int NC, bool GROUPED> __global__ __launch_bounds__(256) void 
     bool keep = true;
     if (a.claim) {
         keep = a.claim[slot] == (int32_t)r;
-        if (keep && l == 0 && a.segs == 1) a.claim[slot] = -1;   // (a frame that lost reads its rival's index or this: neither is its own)
+        if (keep && l == 0 && a.p.segs == 1) a.claim[slot] = -1;   // (a frame that lost reads its rival's index or this: neither is its own)
     } else if (a.slots.at && a.n > 1) {
         bool again = false;
         for (int64_t i = r + 1 + l; i < a.n; i += lanes) again |= a.slots.at[i] == slot;
@@ -296,7 +316,7 @@ template <class T, int NC, bool GROUPED> __global__ __launch_bounds__(256) void 
             *(float2*)(row + a.l.scale_off + 8 * (GROUPED ? ug >> a.gunits_log2 : 0)) = make_float2(s.lo, s.step);
 #pragma unroll
         for (int k = GROUPED ? g : 0; k < (GROUPED ? g + 1 : NC); k++)
-            if (n[k] > 0) put_unit<T>(a, row, y, keep, u0 + l + k * lanes, n[k], w[k], s, per);
+            if (n[k] > 0) put_unit<T, S>(a, row, y, keep, u0 + l + k * lanes, n[k], w[k], s, per);
     }
 }
 
@@ -327,7 +347,7 @@ template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs
     int flags = 0;
     for (int c = t * UV<T>; c < cols; c += 256 * UV<T>) {
         const int n = min(UV<T>, cols - c);
-        const Unit<T> in = Unit<T>::load(x + c, n);
+        const Unit<T> in = Unit<T>::template load<false>(x + c, n);
 #pragma unroll
         for (int j = 0; j < UV<T>; j++) if (j < n) add_finite(widen(in.v[j]), &mn, &mx, &flags);
     }
@@ -342,84 +362,126 @@ template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs
     if (keep && t == 0) *(float2*)(row + a.l.scale_off) = make_float2(s.lo, s.step);
     for (int c = t * UV<T>; c < cols; c += 256 * UV<T>) {
         const int n = min(UV<T>, cols - c);
-        const Unit<T> in = Unit<T>::load(x + c, n);
+        const Unit<T> in = Unit<T>::template load<false>(x + c, n);
         W w[UV<T>];
 #pragma unroll
         for (int j = 0; j < UV<T>; j++) w[j] = j < n ? widen(in.v[j]) : W(0);
-        put_unit<T>(a, row, y, keep, c / UV<T>, n, w, s, per);
+        put_unit<T, false>(a, row, y, keep, c / UV<T>, n, w, s, per);
     }
 }
 
 // The 32 random bits of the N elements from `e` on: one word of the generator for two elements, its argument stepped from word to word;
-// an odd start straddles words and needs one more.  The word's index has 63 bits, so where the element's 64 wrap to zero the step
-// would be wrong: elements that may be there take their words one by one.
-template <int N> GL_DEV void random_bits(uint64_t seed, uint64_t e, uint32_t* u) {
+// an odd start straddles words and needs one more.  The word's index has 63 bits: where the element's 64 wrap to zero (`wraps`: the call
+// reaches there) the stepped argument is 2^63 kGamma = 2^63 too large.
+template <int N> GL_DEV void random_bits(uint64_t seed, uint64_t e, bool wraps, uint32_t* u) {
     const uint64_t i = e >> 1;
-    uint64_t z = seed + (i + 1) * kGamma;
-    if ((uint32_t)(i >> 32) == 0x7FFFFFFFu) {
+    const bool odd = e & 1;
+    uint64_t z[N / 2 + 1], w[N / 2 + 1];
+    z[0] = seed + (i + 1) * kGamma;
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const uint64_t at = e + (uint32_t)j, w = splitmix_of(seed + ((at >> 1) + 1) * kGamma);
-            u[j] = (uint32_t)((at & 1) ? w >> 32 : w);
-        }
-    } else if (!(e & 1)) {
+    for (int j = 1; j <= N / 2; j++) z[j] = z[j - 1] + kGamma;
+    if (wraps) {
 #pragma unroll
-        for (int j = 0; j < N; j += 2, z += kGamma) {
-            const uint64_t w = splitmix_of(z);
-            u[j] = (uint32_t)w;
-            u[j + 1] = (uint32_t)(w >> 32);
-        }
-    } else {
-        uint32_t before = (uint32_t)(splitmix_of(z) >> 32);
+        for (int j = 1; j <= N / 2; j++) z[j] ^= (i + j) & ((uint64_t)1 << 63);
+    }
 #pragma unroll
-        for (int j = 0; j < N; j += 2) {
-            z += kGamma;
-            const uint64_t w = splitmix_of(z);
-            u[j] = before;
-            u[j + 1] = (uint32_t)w;
-            before = (uint32_t)(w >> 32);
-        }
+    for (int j = 0; j < N / 2; j++) w[j] = splitmix_of(z[j]);
+    w[N / 2] = 0;
+    if (odd) w[N / 2] = splitmix_of(z[N / 2]);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        u[j] = odd ? (uint32_t)(w[j / 2] >> 32) : (uint32_t)w[j / 2];
+        u[j + 1] = odd ? (uint32_t)w[j / 2 + 1] : (uint32_t)(w[j / 2] >> 32);
     }
 }
-template <class T> GL_DEV void drop_unit(Unit<T>* x, const DropRule& d, const uint32_t* u) {
+template <class T> GL_DEV T drop_or(typename Wide<T>::type v, const DropRule& d, uint32_t u) {
     typedef typename Wide<T>::type W;
-#pragma unroll
-    for (int j = 0; j < UV<T>; j++) x->v[j] = narrow<T>(((uint32_t)d.all | (uint32_t)(u[j] < d.below)) ? W(0) : widen(x->v[j]) * (W)d.scale);
+    const bool all = d.all != 0, low = u < d.below;
+    return narrow<T>((all | low) ? W(0) : v * (W)d.scale);
 }
 
-// One unit of the output per lane: its codes (2 ... 8 bytes), its group's scale, one 16-byte store.  Bound by HBM, most of it the output's
-// writing.
-template <class T, int BITS, bool DROP> __global__ __launch_bounds__(512) void k_read(ReadArgs a) {
-    typedef typename Wide<T>::type W;
-    int64_t r, u64;
-    if (!walk_unit(a.w, &r, &u64)) return;
-    const int u = (int)u64, c = u * UV<T>, n = min(UV<T>, 2 * a.l.K - c);
-    const int64_t slot = slot_of(a.slots, r);
+// What k_read and k_read_drop share: the frame this lane works on, its first unit there, the frame's row in the cache; false: none.
+GL_DEV bool read_place(const ReadArgs& a, int units, int64_t* r, int* u0, const uint8_t** row) {
+    const int lanes = 1 << a.p.lanes_log2, l = (int)threadIdx.x & (lanes - 1);
+    const int64_t part = (int64_t)blockIdx.x * (256 >> a.p.lanes_log2) + ((int)threadIdx.x >> a.p.lanes_log2);
+    if (part >= a.n * a.p.segs) return false;
+    *r = a.p.segs == 1 ? part : part / a.p.segs;
+    *u0 = (a.p.segs == 1 ? 0 : (int)(part - *r * a.p.segs) * (units * lanes)) + l;
+    const int64_t slot = slot_of(a.slots, *r);
     if (slot < 0 || slot >= a.slots.n_slots) {
-        if ((slot >= a.slots.n_slots || a.strict) && u == 0) atomicAdd(a.bad, 1ull);
-        return;
+        if ((slot >= a.slots.n_slots || a.strict) && *u0 == 0) atomicAdd(a.bad, 1ull);
+        return false;
     }
-    const uint8_t* row = a.store + slot * a.l.row_bytes;
-    constexpr int CB = UV<T> * BITS / 8;   // a row's codes are padded to 16 bytes: a partial unit's are there too
-    uint32_t code[CB > 4 ? 2 : 1];
-    code[0] = 0;
-    __builtin_memcpy(code, __builtin_assume_aligned(row + (int64_t)u * CB, CB), CB);
-    const float2 f = *(const float2*)(row + a.l.scale_off + 8 * ((c >> 1) >> a.gshift));
-    const Scale s{f.x, f.y};
-    uint32_t bits[UV<T>];
-    if (DROP) {
-        const uint64_t e = a.offset + (uint64_t)r * (uint32_t)(2 * a.l.K) + (uint32_t)c;
-        random_bits<UV<T>>(a.seed, e, bits);
+    *row = a.store + slot * a.l.row_bytes;
+    return true;
+}
+// A unit's codes: a row's are padded to 16 bytes, so a partial unit's are there too.
+template <class T, int BITS> struct Codes {
+    static constexpr int bytes = UV<T> * BITS / 8;
+    uint32_t v[bytes > 4 ? 2 : 1];
+    __device__ __forceinline__ void load(const uint8_t* row, int u) {
+        v[0] = 0;
+        __builtin_memcpy(v, __builtin_assume_aligned(row + u * bytes, bytes), bytes);
     }
-    Unit<T> out;
+    __device__ __forceinline__ float at(int j) const { return (float)(v[j * BITS / 32] >> (j * BITS % 32) & ((1u << BITS) - 1)); }
+};
+
+// A frame over the lanes as in k_write.  Per unit: its codes (1 ... 8 bytes), its group's scale, one 16-byte store.
+template <class T, int BITS, int NC, bool S> __global__ __launch_bounds__(256) void k_read(ReadArgs a) {
+    typedef typename Wide<T>::type W;
+    int64_t r;
+    int u0;
+    const uint8_t* row;
+    if (!read_place(a, NC, &r, &u0, &row)) return;
+    const int lanes = 1 << a.p.lanes_log2;
+    const float2* scales = (const float2*)(row + a.l.scale_off);
+    Codes<T, BITS> code[NC];
+    float2 f[NC];
+    int n[NC];
 #pragma unroll
-    for (int j = 0; j < UV<T>; j++) {
-        const uint32_t q = code[j * BITS / 32] >> (j * BITS % 32) & ((1u << BITS) - 1);
-        W v = dequantise((float)q, s, W(0));
-        if (DROP) v = ((uint32_t)a.drop.all | (uint32_t)(bits[j] < a.drop.below)) ? W(0) : v * (W)a.drop.scale;
-        out.v[j] = narrow<T>(v);
+    for (int k = 0; k < NC; k++) {
+        const int u = u0 + k * lanes;
+        n[k] = min(UV<T>, 2 * a.l.K - u * UV<T>);
+        if (n[k] <= 0) continue;
+        code[k].load(row, u);
+        f[k] = scales[(u * UV<T> >> 1) >> a.gshift];
     }
-    out.store((T*)a.y + r * a.ys + c, n);
+    T* y = (T*)a.y + r * a.ys;
+#pragma unroll
+    for (int k = 0; k < NC; k++) {
+        if (n[k] <= 0) continue;
+        Unit<T> out;
+#pragma unroll
+        for (int j = 0; j < UV<T>; j++) out.v[j] = narrow<T>(dequantise(code[k].at(j), Scale{f[k].x, f[k].y}, W(0)));
+        out.template store<S>(y + (u0 + k * lanes) * UV<T>, n[k]);
+    }
+}
+// The same with dropout: bound by the generator as dropout alone is, so the lane's units go through one loop body.
+template <class T, int BITS, bool S> __global__ __launch_bounds__(256) void k_read_drop(ReadArgs a) {
+    typedef typename Wide<T>::type W;
+    int64_t r;
+    int u0;
+    const uint8_t* row;
+    if (!read_place(a, a.p.units, &r, &u0, &row)) return;
+    const float2* scales = (const float2*)(row + a.l.scale_off);
+    T* y = (T*)a.y + r * a.ys;
+    const uint64_t e = a.offset + (uint64_t)r * (uint32_t)(2 * a.l.K);
+#pragma unroll 1
+    for (int k = 0; k < a.p.units; k++) {
+        const int c = (u0 + (k << a.p.lanes_log2)) * UV<T>, n = min(UV<T>, 2 * a.l.K - c);
+        if (n <= 0) return;
+        Codes<T, BITS> code;
+        code.load(row, c / UV<T>);
+        const float2 f = scales[(c >> 1) >> a.gshift];
+        uint32_t bits[UV<T>];
+        random_bits<UV<T>>(a.seed, e + (uint32_t)c, a.wraps, bits);
+        Unit<T> out;
+#pragma unroll
+        for (int j = 0; j < UV<T>; j++) {
+            out.v[j] = drop_or<T>(dequantise(code.at(j), Scale{f.x, f.y}, W(0)), a.drop, bits[j]);
+        }
+        out.template store<S>(y + c, n);
+    }
 }
 
 struct DropArgs {
@@ -428,33 +490,36 @@ struct DropArgs {
     Walk w;
     DropRule drop;
     uint64_t seed, offset;
+    int32_t wraps;            // offset + total pass 2^64
 };
 // Dense arrays: one unit per lane.  Bound by HBM in fp32 and fp64 (two streams), by the generator's multiplications in the 16-bit types:
 // six quarter-rate 32-bit products for two elements.  One unit per lane is the best of 1, 2, 4 and 8: with more in flight per lane
 // fp32 falls from 6.17 to 5.9 TB/s, bf16 from 6.08 to 5.8 (409 600 x 384 elements, bytes read and written).
-template <class T> __global__ __launch_bounds__(256) void k_dropout(DropArgs a) {
+template <class T, bool S, bool LN> __global__ __launch_bounds__(256) void k_dropout(DropArgs a) {
     const int64_t e0 = (int64_t)blockIdx.x * (256 * UV<T>);
     const int t = (int)threadIdx.x * UV<T>;
     const int n = (int)min((int64_t)UV<T>, a.total - e0 - t);
     if (n <= 0) return;
-    Unit<T> x = Unit<T>::load((const T*)a.x + e0 + t, n);
+    Unit<T> x = Unit<T>::template load<LN>((const T*)a.x + e0 + t, n);
     uint32_t u[UV<T>];
-    random_bits<UV<T>>(a.seed, a.offset + (uint64_t)e0 + (uint32_t)t, u);
-    drop_unit(&x, a.drop, u);
-    x.store((T*)a.y + e0 + t, n);
+    random_bits<UV<T>>(a.seed, a.offset + (uint64_t)e0 + (uint32_t)t, a.wraps, u);
+#pragma unroll
+    for (int j = 0; j < UV<T>; j++) x.v[j] = drop_or<T>(widen(x.v[j]), a.drop, u[j]);
+    x.template store<S>((T*)a.y + e0 + t, n);
 }
 // Rows apart.
-template <class T> __global__ __launch_bounds__(512) void k_dropout_rows(DropArgs a) {
+template <class T, bool S> __global__ __launch_bounds__(512) void k_dropout_rows(DropArgs a) {
     int64_t r, k;
     if (!walk_unit(a.w, &r, &k)) return;
     const int64_t c = k * UV<T>;
     const int n = (int)min((int64_t)UV<T>, a.cols - c);
-    Unit<T> x = Unit<T>::load((const T*)a.x + r * a.xs + c, n);
+    Unit<T> x = Unit<T>::template load<false>((const T*)a.x + r * a.xs + c, n);
     const uint64_t e = a.offset + (uint64_t)(r * a.cols + c);
     uint32_t u[UV<T>];
-    random_bits<UV<T>>(a.seed, e, u);
-    drop_unit(&x, a.drop, u);
-    x.store((T*)a.y + r * a.ys + c, n);
+    random_bits<UV<T>>(a.seed, e, a.wraps, u);
+#pragma unroll
+    for (int j = 0; j < UV<T>; j++) x.v[j] = drop_or<T>(widen(x.v[j]), a.drop, u[j]);
+    x.template store<S>((T*)a.y + r * a.ys + c, n);
 }
 
 #define GL_TYPES(type, ...)                                          \
@@ -464,16 +529,42 @@ template <class T> __global__ __launch_bounds__(512) void k_dropout_rows(DropArg
         case GOMEL_F16: { typedef __half T; __VA_ARGS__; } break;    \
         default: { typedef __hip_bfloat16 T; __VA_ARGS__; } break;   \
     }
-template <class T> void (*write_kernel(int units, bool grouped))(WriteArgs) {
+template <class T, bool G, bool S> void (*write_kernel(int units))(WriteArgs) {
     switch (units) {
-        case 1: return grouped ? k_write<T, 1, true> : k_write<T, 1, false>;
-        case 2: return grouped ? k_write<T, 2, true> : k_write<T, 2, false>;
-        case 3: return grouped ? k_write<T, 3, true> : k_write<T, 3, false>;
-        case 4: return grouped ? k_write<T, 4, true> : k_write<T, 4, false>;
-        case 5: return grouped ? k_write<T, 5, true> : k_write<T, 5, false>;
-        default: return grouped ? k_write<T, 6, true> : k_write<T, 6, false>;
+        case 1: return k_write<T, 1, G, S>;
+        case 2: return k_write<T, 2, G, S>;
+        case 3: return k_write<T, 3, G, S>;
+        case 4: return k_write<T, 4, G, S>;
+        case 5: return k_write<T, 5, G, S>;
+        default: return k_write<T, 6, G, S>;
     }
 }
+template <class T> void (*write_kernel(int units, bool grouped, bool streamed))(WriteArgs) {
+    if (grouped) return streamed ? write_kernel<T, true, true>(units) : write_kernel<T, true, false>(units);
+    return streamed ? write_kernel<T, false, true>(units) : write_kernel<T, false, false>(units);
+}
+template <class T, int BITS, bool S> void (*read_kernel(int units, bool dropping))(ReadArgs) {
+    if (dropping) return k_read_drop<T, BITS, S>;
+    switch (units) {
+        case 1: return k_read<T, BITS, 1, S>;
+        case 2: return k_read<T, BITS, 2, S>;
+        case 3: return k_read<T, BITS, 3, S>;
+        case 4: return k_read<T, BITS, 4, S>;
+        case 5: return k_read<T, BITS, 5, S>;
+        default: return k_read<T, BITS, 6, S>;
+    }
+}
+template <class T> void (*read_kernel(int bits, int units, bool dropping, bool streamed))(ReadArgs) {
+    if (bits == 8) return streamed ? read_kernel<T, 8, true>(units, dropping) : read_kernel<T, 8, false>(units, dropping);
+    return streamed ? read_kernel<T, 4, true>(units, dropping) : read_kernel<T, 4, false>(units, dropping);
+}
+// Large outputs are stored past the caches (non-temporal): left in them, their write-back is in the way of the kernels that follow.  A
+// read of 102 400 x 192 bands (157 MB of fp32) takes 28.4 us instead of 45.3, 50.7 instead of 94.7 in fp64, a write with its values 62
+// instead of 80, dropout of 79 MB of bf16 23.8 instead of 29.0, each among others of its kind; with a consumer right behind that could
+// have found the output in the 256 MB last-level cache, the pair gains (write, dropout: up to 9 %) or loses (read: up to 5 %).  Below a
+// quarter of that cache nothing is gained.  Frames to be written are loaded so too, dropout's input where input and output together do
+// not fit (315 MB of fp32: 194.9 instead of 199.2 us; 79 MB: 26.7 instead of 23.8).
+constexpr size_t kStreamBytes = (size_t)64 << 20, kStreamInBytes = (size_t)128 << 20;
 // launches report their own status: hipGetLastError could hand back somebody else's
 template <class Args> hipError_t launch(void (*k)(Args), unsigned grid, unsigned block, hipStream_t s, Args& a) {
     void* p[] = {&a};
@@ -505,24 +596,24 @@ bool capturing(hipStream_t s) {
 }
 
 hipError_t dropout_device(int type, const void* x, size_t xs, void* y, size_t ys, size_t rows, size_t cols, const DropRule& d, uint64_t seed, uint64_t offset, hipStream_t s) {
-    const size_t total = rows * cols, uv = 16 / (size_t)type_bytes(type);
-    DropArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)cols, (int64_t)total, Walk{}, d, seed, offset};
+    const size_t total = rows * cols, bytes = total * (size_t)type_bytes(type), uv = 16 / (size_t)type_bytes(type);
+    DropArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)cols, (int64_t)total, Walk{}, d, seed, offset, (int32_t)(offset + (uint64_t)total < offset)};
     hipError_t e = hipSuccess;
     if ((xs == cols && ys == cols) || rows == 1) {
         const size_t units = (total + uv - 1) / uv, blocks = (units + 256 - 1) / 256;
         if (blocks > INT32_MAX) return hipErrorInvalidValue;
-        GL_TYPES(type, e = launch(k_dropout<T>, (unsigned)blocks, 256, s, a));
+        GL_TYPES(type, e = launch(bytes < kStreamBytes ? k_dropout<T, false, false> : bytes < kStreamInBytes ? k_dropout<T, true, false> : k_dropout<T, true, true>,
+                                  (unsigned)blocks, 256, s, a));
         return e;
     }
     a.w = walk_of(rows, (cols + uv - 1) / uv);
     if (a.w.blocks > INT32_MAX) return hipErrorInvalidValue;
-    GL_TYPES(type, e = launch(k_dropout_rows<T>, (unsigned)a.w.blocks, (unsigned)a.w.block, s, a));
+    GL_TYPES(type, e = launch(bytes < kStreamBytes ? k_dropout_rows<T, false> : k_dropout_rows<T, true>, (unsigned)a.w.blocks, (unsigned)a.w.block, s, a));
     return e;
 }
 
 constexpr size_t kStageBytes = (size_t)32 << 20;
 constexpr size_t kScanRows = 2048;   // frames of a write up to which each looks through the later slots itself; more claim theirs first
-constexpr int kMostUnits = 6;        // units a lane of k_write holds
 
 // Rows between host memory (stride elements apart) and a dense device buffer
 hipError_t rows_in(void* dev, const char* host, size_t stride, size_t rows, size_t cols, size_t esz, hipStream_t s) {
@@ -675,32 +766,23 @@ int memory_kind(const void* p, int device) {
 }
 
 hipError_t cache_write_device(gomel_cache* c, int type, const void* x, size_t xs, size_t n, const int64_t* slots, size_t first, void* y, size_t ys, hipStream_t s) {
-    const bool claims = slots && n > kScanRows;
-    WriteArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, claims ? c->claim : nullptr, c->bad, 6, 0, 1};
+    const bool claims = slots && n > kScanRows, grouped = c->l.groups > 1;
     const int uv = 16 / type_bytes(type), upr = (2 * c->l.K + uv - 1) / uv;
-    const bool grouped = c->l.groups > 1;
-    int least_lanes = 3, nc = 0;
-    if (grouped) {
-        while ((uv << a.gunits_log2) < 2 * c->l.group) a.gunits_log2++;
-        least_lanes = std::max(least_lanes, a.gunits_log2);
-    }
-    // lanes x units per lane: the pair with the fewest idle places, the most lanes among equals
-    for (int lg = 6, best = INT32_MAX; lg >= least_lanes; lg--) {
-        const int k = (upr + (1 << lg) - 1) >> lg;
-        if (k <= kMostUnits && (k << lg) < best) { best = k << lg; nc = k; a.lanes_log2 = lg; }
-    }
+    int gunits_log2 = 0;
+    if (grouped) while ((uv << gunits_log2) < 2 * c->l.group) gunits_log2++;
+    WriteArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, claims ? c->claim : nullptr, c->bad,
+                spread_of(upr, std::max(3, gunits_log2), grouped), gunits_log2};
     hipError_t e = hipSuccess;
     if (claims) e = launch_claim(k_claim, a.slots, a.n, c->claim, s);
     if (e != hipSuccess) return e;
-    if (!nc && !grouped) {
+    if (!a.p.units) {
         GL_TYPES(type, e = launch(k_write_wide<T>, (unsigned)n, 256, s, a));
         return e;
     }
-    if (!nc) { nc = 4; a.segs = (upr + 255) / 256; }   // wide and grouped: segments of 64 lanes x 4 units, whole groups each
-    const size_t per = 256 >> a.lanes_log2, blocks = (n * (size_t)a.segs + per - 1) / per;
+    const size_t per = 256 >> a.p.lanes_log2, blocks = (n * (size_t)a.p.segs + per - 1) / per;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    GL_TYPES(type, e = launch(write_kernel<T>(nc, grouped), (unsigned)blocks, 256, s, a));
-    if (claims && a.segs > 1 && e == hipSuccess) e = launch_claim(k_claim_clear, a.slots, a.n, c->claim, s);
+    GL_TYPES(type, e = launch(write_kernel<T>(a.p.units, grouped, 2 * (size_t)c->l.K * n * type_bytes(type) >= kStreamBytes), (unsigned)blocks, 256, s, a));
+    if (claims && a.p.segs > 1 && e == hipSuccess) e = launch_claim(k_claim_clear, a.slots, a.n, c->claim, s);
     return e;
 }
 
@@ -709,13 +791,13 @@ hipError_t cache_read_device(gomel_cache* c, int type, void* y, size_t ys, size_
     const int uv = 16 / type_bytes(type);
     int gshift = 31;
     if (c->l.groups > 1) for (gshift = 0; (1 << gshift) < c->l.group; gshift++) {}
-    ReadArgs a{y, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, walk_of(n, (size_t)(2 * c->l.K + uv - 1) / uv), drop,
-               gshift, (int32_t)strict, seed, offset, bad ? bad : c->bad};
-    if (a.w.blocks > INT32_MAX) return hipErrorInvalidValue;
-    const bool wide = c->l.bits == 8, dropping = drop.all || drop.below != 0;
+    ReadArgs a{y, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, spread_of((2 * c->l.K + uv - 1) / uv, 3, true), drop,
+               gshift, (int32_t)strict, seed, offset, bad ? bad : c->bad, (int32_t)(offset + 2 * (uint64_t)c->l.K * n < offset)};
+    const size_t per = 256 >> a.p.lanes_log2, blocks = (n * (size_t)a.p.segs + per - 1) / per;
+    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    const bool dropping = drop.all || drop.below != 0;
     hipError_t e = hipSuccess;
-    GL_TYPES(type, e = launch(dropping ? (wide ? k_read<T, 8, true> : k_read<T, 4, true>) : (wide ? k_read<T, 8, false> : k_read<T, 4, false>),
-                              (unsigned)a.w.blocks, (unsigned)a.w.block, s, a));
+    GL_TYPES(type, e = launch(read_kernel<T>(c->l.bits, a.p.units, dropping, 2 * (size_t)c->l.K * n * type_bytes(type) >= kStreamBytes), (unsigned)blocks, 256, s, a));
     return e;
 }
 
