@@ -12,6 +12,7 @@ from . import _lib
 from ._lib import check
 from .mel import Batch, DevicePointer
 
+_ON_DEVICE = 0x100           # GOMEL_DEVICE_MEMORY: nothing of the call is in host memory
 _TYPES = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}
 _torch = None                # the module, once a tensor has been seen
 _Tensor = None               # its Tensor type
@@ -171,7 +172,10 @@ class Cache:
                 raise ValueError("values: the frames' type and number of frames are needed")
         if first < 0:
             raise ValueError("first is negative")
-        rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, _device_of(self.device, dev, vdev, sdev)))
+        on = _device_of(self.device, dev, vdev, sdev)
+        if on == self.device and dev is not None and (values is None or vdev is not None) and (slots is None or sdev is not None):
+            t |= _ON_DEVICE
+        rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, on))
         if rc:
             check(rc, "gomel_cache_write")
         return values
@@ -183,8 +187,10 @@ class Cache:
         sp, keep, sdev = (0, None, None) if slots is None else _slots(slots, n)
         if first < 0:
             raise ValueError("first is negative")
-        rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
-                        _stream(stream, _device_of(self.device, dev, sdev)))
+        on = _device_of(self.device, dev, sdev)
+        if on == self.device and dev is not None and (slots is None or sdev is not None):
+            t |= _ON_DEVICE
+        rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on))
         if rc:
             check(rc, "gomel_cache_read")
         return out
@@ -263,6 +269,15 @@ def _flat(a, what, write=False):
 
 
 def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
+    device = engine.cfg.device
+    if out is not None and _is_tensor(x) and _is_tensor(out) and x.is_contiguous() and out.is_contiguous() and x.shape == out.shape and x.dtype == out.dtype:
+        t, n = _torch_types.get(x.dtype), x.numel()                       # two dense tensors: nothing to work out
+        if t is not None and n and device == x.get_device() == out.get_device():
+            rc = fn(engine._h, t | _ON_DEVICE, x.data_ptr(), n, out.data_ptr(), n, 1, n, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
+                    _stream(stream, device))
+            if rc:
+                check(rc, where)
+            return out
     ptr, t, xs, rows, cols, dev = _flat(x, "x")
     if out is None:
         if isinstance(x, DevicePointer):
@@ -276,8 +291,10 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
             rows, cols, xs = orows, ocols, ocols
         else:
             os_ = cols
-    rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
-            _stream(stream, _device_of(engine.cfg.device, dev, odev)))
+    on = _device_of(device, dev, odev)
+    if on == device and dev is not None and odev is not None:
+        t |= _ON_DEVICE
+    rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on))
     if rc:
         check(rc, where)
     return out

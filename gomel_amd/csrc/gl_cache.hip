@@ -100,11 +100,15 @@ template <class T> struct Unit {
 
 // How a frame lies over a wave: in 2^lanes_log2 neighbouring lanes, `units` units each, `lanes` apart, so that every access of the wave is
 // one run of memory and what depends on the frame alone (its slot, its addresses) is worked out once per lane.  A frame too wide for
-// that is cut into `segs` segments of 64 lanes x 4 units (units = 0: k_write cannot, it needs the extremes of the whole frame).
+// that is cut into `segs` segments of 64 lanes x 4 units (units = 0: k_write cannot, it needs the extremes of the whole frame).  Up to
+// kSpreadRows frames a wave each fits the chip: then all 64 lanes, and the fewest units after each other (a write of 64 frames of 160
+// bands in fp16: 5.6 us with 64 lanes x 1 unit, 8.6 with 8 x 5).
 struct Spread { int32_t lanes_log2, units, segs; };
 constexpr int kMostUnits = 6;
-inline Spread spread_of(int upr, int least_lanes_log2, bool may_cut) {
+constexpr size_t kSpreadRows = 4096;
+inline Spread spread_of(size_t n, int upr, int least_lanes_log2, bool may_cut) {
     Spread p{6, 0, 1};
+    if (n <= kSpreadRows) least_lanes_log2 = 6;
     // the pair with the fewest idle places, the most lanes among equals
     for (int lg = 6, best = INT32_MAX; lg >= least_lanes_log2; lg--) {
         const int k = (upr + (1 << lg) - 1) >> lg;
@@ -279,7 +283,13 @@ template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(25
         if (keep && l == 0 && a.p.segs == 1) a.claim[slot] = -1;   // (a frame that lost reads its rival's index or this: neither is its own)
     } else if (a.slots.at && a.n > 1) {
         bool again = false;
-        for (int64_t i = r + 1 + l; i < a.n; i += lanes) again |= a.slots.at[i] == slot;
+        for (int i = (int)r + 1 + l; i < (int)a.n; i += 8 * lanes) {   // eight loads in flight: one at a time costs 0.1 us each
+            int64_t at[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) at[k] = a.slots.at[min(i + k * lanes, (int)a.n - 1)];
+#pragma unroll
+            for (int k = 0; k < 8; k++) again |= at[k] == slot && i + k * lanes < (int)a.n;
+        }
         keep = !(__ballot(again) >> first & (~0ull >> (64 - lanes)));
     }
     uint8_t* row = a.store + slot * a.l.row_bytes;
@@ -613,7 +623,9 @@ hipError_t dropout_device(int type, const void* x, size_t xs, void* y, size_t ys
 }
 
 constexpr size_t kStageBytes = (size_t)32 << 20;
-constexpr size_t kScanRows = 2048;   // frames of a write up to which each looks through the later slots itself; more claim theirs first
+// Frames of a write up to which each looks through the later slots itself, per lane that looks; more claim theirs first.  The search grows
+// with the square (192 bands of bf16, 16 lanes: 6.4 us for 256 frames, 8.0 for 1024, 10.2 for 2048), the claims cost a launch (8.8 ... 9.1).
+constexpr size_t kScanPerLane = 64;
 
 // Rows between host memory (stride elements apart) and a dense device buffer
 hipError_t rows_in(void* dev, const char* host, size_t stride, size_t rows, size_t cols, size_t esz, hipStream_t s) {
@@ -645,6 +657,8 @@ int check_slots(const int64_t* slots, size_t n, size_t n_slots, bool pad_ok) {
 // through the staging buffer in pieces.  `in` (write only) and `out` (write: values, may be null) are rows `is` / `os` elements apart.
 template <class Run>
 int cache_call(gomel_cache* c, int type, const void* in, size_t is, void* out, size_t os, size_t n, const int64_t* slots, size_t first, hipStream_t s, Run run) {
+    const bool vouched = type & GOMEL_DEVICE_MEMORY;
+    type &= ~GOMEL_DEVICE_MEMORY;
     const size_t cols = 2 * (size_t)c->l.K, esz = (size_t)type_bytes(type);
     if (!esz) return GOMEL_ERR_BAD_CONFIG;
     if (n == 0) return GOMEL_OK;
@@ -652,9 +666,10 @@ int cache_call(gomel_cache* c, int type, const void* in, size_t is, void* out, s
     if (!slots && (first > c->n_slots || n > c->n_slots - first)) return GOMEL_ERR_TABLE_RANGE;
     if (in && out && !rows_disjoint_or_same(in, is, out, os, n, cols, esz)) return GOMEL_ERR_BAD_CONFIG;
     OnDevice dev(c->device); CHK(dev.err);
+    if (vouched) { CHK(run(type, in, is, out, os, n, slots, first)); return GOMEL_OK; }
     const int ki = in ? memory_kind(in, c->device) : 1, ko = out ? memory_kind(out, c->device) : 1, ks = slots ? memory_kind(slots, c->device) : 1;
     if (ki < 0 || ko < 0 || ks < 0) return GOMEL_ERR_BAD_CONFIG;
-    if (ki && ko && ks) { CHK(run(in, is, out, os, n, slots, first)); return GOMEL_OK; }
+    if (ki && ko && ks) { CHK(run(type, in, is, out, os, n, slots, first)); return GOMEL_OK; }
     if (capturing(s)) return GOMEL_ERR_BAD_CONFIG;
     if (!ks) { const int rc = check_slots(slots, n, c->n_slots, true); if (rc) return rc; }
     std::lock_guard<std::mutex> lk(c->mu);
@@ -673,7 +688,7 @@ int cache_call(gomel_cache* c, int type, const void* in, size_t is, void* out, s
         if (!ks) e = hipMemcpyAsync(st_slots, at, m * 8, hipMemcpyHostToDevice, s);
         if (!ki && e == hipSuccess) e = rows_in(st, from, is, m, cols, esz, s);
         if (!ko && slots && e == hipSuccess) e = rows_in(st_out, to, os, m, cols, esz, s);   // rows of padding come back as they were
-        if (e == hipSuccess) e = run(ki ? from : st, ki ? is : cols, ko ? to : st_out, ko ? os : cols, m, ks ? at : (const int64_t*)st_slots, first + r);
+        if (e == hipSuccess) e = run(type, ki ? from : st, ki ? is : cols, ko ? to : st_out, ko ? os : cols, m, ks ? at : (const int64_t*)st_slots, first + r);
         if (!ko && e == hipSuccess) e = rows_out(to, st_out, os, m, cols, esz, s);
     }
     const hipError_t e2 = hipStreamSynchronize(s);   // also on an error: the staging buffer is free again when the lock goes
@@ -720,6 +735,8 @@ int cache_create(gomel_handle* h, size_t n_slots, int bits, int group_bands, gom
 
 int dropout_call(gomel_handle* h, int type, const void* x, size_t xs, void* y, size_t ys, size_t rows, size_t cols, double p, uint64_t seed, uint64_t offset, hipStream_t s) {
     if (!h) return GOMEL_ERR_NULL;
+    const bool vouched = type & GOMEL_DEVICE_MEMORY;
+    type &= ~GOMEL_DEVICE_MEMORY;
     const size_t esz = (size_t)type_bytes(type);
     DropRule d;
     if (!esz || !drop_rule(p, &d)) return GOMEL_ERR_BAD_CONFIG;
@@ -729,7 +746,7 @@ int dropout_call(gomel_handle* h, int type, const void* x, size_t xs, void* y, s
     if (!rows_disjoint_or_same(x, xs, y, ys, rows, cols, esz)) return GOMEL_ERR_BAD_CONFIG;
     const int device = handle_device(h);
     OnDevice dev(device); CHK(dev.err);
-    const int kx = memory_kind(x, device), ky = memory_kind(y, device);
+    const int kx = vouched ? 1 : memory_kind(x, device), ky = vouched ? 1 : memory_kind(y, device);
     if (kx < 0 || ky < 0) return GOMEL_ERR_BAD_CONFIG;
     if (kx && ky) { CHK(dropout_device(type, x, xs, y, ys, rows, cols, d, seed, offset, s)); return GOMEL_OK; }
     if (capturing(s)) return GOMEL_ERR_BAD_CONFIG;
@@ -766,12 +783,13 @@ int memory_kind(const void* p, int device) {
 }
 
 hipError_t cache_write_device(gomel_cache* c, int type, const void* x, size_t xs, size_t n, const int64_t* slots, size_t first, void* y, size_t ys, hipStream_t s) {
-    const bool claims = slots && n > kScanRows, grouped = c->l.groups > 1;
+    const bool grouped = c->l.groups > 1;
     const int uv = 16 / type_bytes(type), upr = (2 * c->l.K + uv - 1) / uv;
     int gunits_log2 = 0;
     if (grouped) while ((uv << gunits_log2) < 2 * c->l.group) gunits_log2++;
-    WriteArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, claims ? c->claim : nullptr, c->bad,
-                spread_of(upr, std::max(3, gunits_log2), grouped), gunits_log2};
+    const Spread p = spread_of(n, upr, std::max(3, gunits_log2), grouped);
+    const bool claims = slots && n > (p.units ? kScanPerLane << p.lanes_log2 : 2048);
+    WriteArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, claims ? c->claim : nullptr, c->bad, p, gunits_log2};
     hipError_t e = hipSuccess;
     if (claims) e = launch_claim(k_claim, a.slots, a.n, c->claim, s);
     if (e != hipSuccess) return e;
@@ -791,7 +809,7 @@ hipError_t cache_read_device(gomel_cache* c, int type, void* y, size_t ys, size_
     const int uv = 16 / type_bytes(type);
     int gshift = 31;
     if (c->l.groups > 1) for (gshift = 0; (1 << gshift) < c->l.group; gshift++) {}
-    ReadArgs a{y, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, spread_of((2 * c->l.K + uv - 1) / uv, 3, true), drop,
+    ReadArgs a{y, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, spread_of(n, (2 * c->l.K + uv - 1) / uv, 3, true), drop,
                gshift, (int32_t)strict, seed, offset, bad ? bad : c->bad, (int32_t)(offset + 2 * (uint64_t)c->l.K * n < offset)};
     const size_t per = 256 >> a.p.lanes_log2, blocks = (n * (size_t)a.p.segs + per - 1) / per;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
@@ -830,7 +848,7 @@ int gomel_cache_write(gomel_cache* c, int type, const void* frames, size_t strid
     const hipStream_t s = (hipStream_t)stream;
     GOMEL_TRY
     return cache_call(c, type, frames, stride, values, values_stride, n, slots, first, s,
-                      [&](const void* in, size_t is, void* out, size_t os, size_t m, const int64_t* at, size_t f) { return cache_write_device(c, type, in, is, m, at, f, out, os, s); });
+                      [&](int t, const void* in, size_t is, void* out, size_t os, size_t m, const int64_t* at, size_t f) { return cache_write_device(c, t, in, is, m, at, f, out, os, s); });
     GOMEL_CATCH
 }
 
@@ -843,8 +861,8 @@ int gomel_cache_read(gomel_cache* c, int type, void* frames, size_t stride, size
     const uint64_t cols = 2 * (uint64_t)c->l.K;
     GOMEL_TRY
     size_t done = 0;   // frames of earlier pieces: the counter of a piece's first element
-    return cache_call(c, type, nullptr, 0, frames, stride, n, slots, first, s, [&](const void*, size_t, void* out, size_t os, size_t m, const int64_t* at, size_t f) {
-        const hipError_t e = cache_read_device(c, type, out, os, m, at, f, d, seed, offset + done * cols, false, nullptr, s);
+    return cache_call(c, type, nullptr, 0, frames, stride, n, slots, first, s, [&](int t, const void*, size_t, void* out, size_t os, size_t m, const int64_t* at, size_t f) {
+        const hipError_t e = cache_read_device(c, t, out, os, m, at, f, d, seed, offset + done * cols, false, nullptr, s);
         done += m;
         return e;
     });

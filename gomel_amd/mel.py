@@ -367,30 +367,25 @@ class Engine:
     # -- spectrogram cache, dropout ------------------------------------------------------------------
     def cache(self, n_slots, bits=8, group=0):
         """A device-resident cache of `n_slots` quantised frames of this engine's NumMels (gomel_amd.Cache)."""
-        from .cache import Cache
-        return Cache(self, n_slots, bits, group)
+        return _cache.Cache(self, n_slots, bits, group)
 
     def to_mel_cache(self, waves, cache, slots, stream=None):
         """gomel_to_mel_cache: ToMel of every waveform, the frames quantised into `cache` at `slots` (one per frame, in the order of
         the waveforms).  Returns the number of frames of each waveform."""
-        from .cache import to_mel_cache
-        return to_mel_cache(self, waves, cache, slots, stream)
+        return _cache.to_mel_cache(self, waves, cache, slots, stream)
 
     def from_cache(self, cache, slots, x0s=None, seeds=None, stream=None):
         """FromMel of utterances whose frames are held in `cache`: `slots` is one array of slots per utterance.  Returns the waveforms."""
-        from .cache import from_cache
-        return from_cache(self, cache, slots, x0s, seeds, stream)
+        return _cache.from_cache(self, cache, slots, x0s, seeds, stream)
 
     def dropout(self, x, p, seed, offset=0, out=None, stream=None):
         """gomel_dropout: x with each element dropped (0) with probability `p` or scaled by 1 / (1 - p), by the counter-based generator at
         (seed, offset + dense index).  A torch tensor that requires a gradient gets one (the mask is made again, never stored)."""
-        from .cache import dropout
-        return dropout(self, x, p, seed, offset, out, stream)
+        return _cache.dropout(self, x, p, seed, offset, out, stream)
 
     def dropout_backward(self, dy, p, seed, offset=0, out=None, stream=None):
         """gomel_dropout_backward: the gradient of `dropout` with the same (p, seed, offset) from the gradient of its output."""
-        from .cache import dropout_backward
-        return dropout_backward(self, dy, p, seed, offset, out, stream)
+        return _cache.dropout_backward(self, dy, p, seed, offset, out, stream)
 
     # -- FFT test hooks ------------------------------------------------------------------------------
     def rfft_frames(self, frames):
@@ -478,8 +473,7 @@ class Batch:
 
     def upload_cache(self, cache, slots, x0s=None, seeds=None, stream=None):
         """upload with the spectrograms taken from `cache`: `slots` holds one slot per frame of the batch, in order (gomel_batch_upload_cache)."""
-        from .cache import batch_upload_cache
-        batch_upload_cache(self, cache, slots, x0s, seeds, stream)
+        _cache.batch_upload_cache(self, cache, slots, x0s, seeds, stream)
 
     def _x0_args(self, x0s, seeds):
         """(pointer array, keep-alive list, seed array) of an upload."""
@@ -801,3 +795,6 @@ def SaveWav(outputFile, vec, sr):
     """mel/mel.go:167-169."""
     from . import codec
     return codec.dumpwav(outputFile, vec, sr)
+
+
+from . import cache as _cache  # noqa: E402  (at the end: it builds on this module)
