@@ -39,17 +39,54 @@ GL_DEV Scale group_scale(double mn, double mx, int flags, int levels) {
     if ((flags & 1) || (mn > mx && (flags & 6) == 6)) return Scale{__builtin_nanf(""), 0.0f};
     if (mn > mx) return Scale{(flags & 2) ? __builtin_inff() : -__builtin_inff(), 0.0f};
     const float lo = to_f32(mn), hi = to_f32(mx);
-    return Scale{lo, (float)(((double)hi - (double)lo) / (double)levels)};
+    // the quotient by a constant, correctly rounded: the product with the rounded reciprocal, its remainder by multiply-add, one
+    // correction (Markstein 1990); equal to the division on 4e8 pairs of fp32 numbers of every size
+    const double d = (double)hi - (double)lo, over = levels == 255 ? 1.0 / 255.0 : 1.0 / 15.0, q = d * over;
+    return Scale{lo, (float)fma(fma(-q, (double)levels, d), over, q)};
 }
-// The code of v as a number.  In fp64, because neighbouring codes meet at borders that fp32 quotients step over (1 value in 3e4 would get
-// the other code).  `per` = 1 / step (0 where step is 0): the product is within 1e-13 of the quotient, so only a value that close to
-// a border -- and beside it, with room -- needs the division itself.  NaN and infinities: fmaxf / fminf return the number.
-GL_DEV float quantise(double v, Scale s, double per, float levels) {
-    const double d = v - (double)s.lo;
-    double t = d * per, q = rint(t);
-    if (fabs(t - q) > 0.5 - 1e-10) q = rint(d / (double)s.step);
-    return fminf(fmaxf((float)q, 0.0f), levels);
+// The code of v as a number, rint((v - lo) / step) in fp64: neighbouring codes meet at borders that fp32 quotients step over (1 value in 3e4
+// would get the other code).  NaN and infinities: fmaxf / fminf return the number.
+GL_DEV float code_of(double v, Scale s, float levels) {
+    if (!(s.step > 0.0f)) return 0.0f;
+    return fminf(fmaxf((float)rint((v - (double)s.lo) / (double)s.step), 0.0f), levels);
 }
+// The codes of N values at once.  The quotients come from products with 1 / step first, and a value whose product is so near a border that
+// the rounding of difference, reciprocal and product could have carried it across -- `margin` -- sends the lane to the definition.
+//   fp32 (and the 16-bit types): v - lo is off by 2^-24 of itself, v_rcp_f32 by 2^-23, the product by 2^-24: 2^-22 of a quotient of at
+// most `levels` (and a little), so levels * 2^-21 is twice what is needed; one value in 4000 is that near at 8 bits.  fp32 instructions
+// cost what fp64 ones do here, but the definition's take twice as many: a 16-bit write was bound by them.
+//   fp64: 2^-51 of the quotient; 2^-33 is far beyond it and as rare as never.
+// Whatever is not a number in between (an infinite value, a step whose reciprocal fp32 does not hold) fails the comparison and goes there too.
+template <int N> GL_DEV void quantise(const float* v, Scale s, float per, float levels, float* q) {
+    const float limit = 0.5f - levels * 0x1p-21f;
+    bool sure[N], all = true;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const float t = (v[j] - s.lo) * per;
+        q[j] = rintf(t);
+        all &= sure[j] = fabsf(t - q[j]) <= limit;
+    }
+    if (!all) {   // value by value: 16-bit frames meet exact ties (one value in 500 at 8 bits), seldom two in a unit
+#pragma unroll
+        for (int j = 0; j < N; j++) if (!sure[j]) q[j] = code_of((double)v[j], s, levels);
+    }
+}
+template <int N> GL_DEV void quantise(const double* v, Scale s, double per, float levels, float* q) {
+    bool sure[N], all = true;
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const double t = (v[j] - (double)s.lo) * per, r = rint(t);
+        all &= sure[j] = fabs(t - r) <= 0.5 - 0x1p-33;
+        q[j] = fminf(fmaxf((float)r, 0.0f), levels);
+    }
+    if (!all) {
+#pragma unroll
+        for (int j = 0; j < N; j++) if (!sure[j]) q[j] = code_of(v[j], s, levels);
+    }
+}
+// 1 / step for them: 0 for step = 0 (all codes are 0), NaN where v_rcp_f32 would return 0 for a step whose reciprocal is subnormal.
+GL_DEV float reciprocal(Scale s, float) { return s.step > 0.0f ? (s.step < 0x1p126f ? __builtin_amdgcn_rcpf(s.step) : __builtin_nanf("")) : 0.0f; }
+GL_DEV double reciprocal(Scale s, double) { return s.step > 0.0f ? 1.0 / (double)s.step : 0.0; }
 GL_DEV float dequantise(float q, Scale s, float) { return fmaf(q, s.step, s.lo); }
 GL_DEV double dequantise(float q, Scale s, double) { return fma((double)q, (double)s.step, (double)s.lo); }
 
@@ -206,16 +243,31 @@ __global__ void k_claim_clear(Slots s, int64_t n, int32_t* claim) {
     if (slot >= 0 && slot < s.n_slots) claim[slot] = -1;
 }
 
-// Extremes of a group while they are being gathered: `odd` turns NaN once a value is not finite.
-template <class W> struct Range {
-    W mn = (W)__builtin_inf(), mx = -(W)__builtin_inf(), odd = 0;
-    __device__ __forceinline__ void add(float v) { mn = fminf(mn, v); mx = fmaxf(mx, v); odd = fmaf(v, 0.0f, odd); }
-    __device__ __forceinline__ void add(double v) { mn = fmin(mn, v); mx = fmax(mx, v); odd = fma(v, 0.0, odd); }
-};
-GL_DEV float least(float a, float b) { return fminf(a, b); }
+// Extremes of a group while they are being gathered.  fp32: gfx950's three-operand minimum and maximum, one instruction for two values, which
+// hand a NaN on: what is not finite shows in the extremes themselves.  fp64: `odd` turns NaN.
+GL_DEV float least(float a, float b) { asm("v_minimum3_f32 %0, %0, %1, %1" : "+v"(a) : "v"(b)); return a; }
+GL_DEV float most(float a, float b) { asm("v_maximum3_f32 %0, %0, %1, %1" : "+v"(a) : "v"(b)); return a; }
 GL_DEV double least(double a, double b) { return fmin(a, b); }
-GL_DEV float most(float a, float b) { return fmaxf(a, b); }
 GL_DEV double most(double a, double b) { return fmax(a, b); }
+template <class W> struct Range;
+template <> struct Range<float> {
+    float mn = __builtin_inff(), mx = -__builtin_inff();
+    __device__ __forceinline__ void add(float a, float b) {
+        asm("v_minimum3_f32 %0, %0, %1, %2" : "+v"(mn) : "v"(a), "v"(b));
+        asm("v_maximum3_f32 %0, %0, %1, %2" : "+v"(mx) : "v"(a), "v"(b));
+    }
+    // (a lane that has added nothing: mn = +inf, mx = -inf)
+    __device__ __forceinline__ bool special() const { return !(mn > -__builtin_inff() && mx < __builtin_inff()); }
+};
+template <> struct Range<double> {
+    double mn = __builtin_inf(), mx = -__builtin_inf(), odd = 0;
+    __device__ __forceinline__ void add(double a, double b) {
+        mn = fmin(mn, fmin(a, b));
+        mx = fmax(mx, fmax(a, b));
+        odd = fma(a, 0.0, fma(b, 0.0, odd));
+    }
+    __device__ __forceinline__ bool special() const { return !(odd == 0.0); }
+};
 // The same with the finite values only, and what the others are (group_scale's flags).
 template <class W> GL_DEV void add_finite(W v, W* mn, W* mx, int* flags) {
     if (v != v) *flags |= 1;
@@ -223,18 +275,16 @@ template <class W> GL_DEV void add_finite(W v, W* mn, W* mx, int* flags) {
     else if (v == -(W)__builtin_inf()) *flags |= 4;
     else { *mn = least(*mn, v); *mx = most(*mx, v); }
 }
-GL_DEV double reciprocal(Scale s) { return s.step > 0.0f ? 1.0 / (double)s.step : 0.0; }
 
 // One unit's codes into the row and, when they are asked for, its values.
-template <class T, bool S> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row, T* y, bool keep, int u, int n, const typename Wide<T>::type* w, Scale s, double per) {
+template <class T, bool S> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row, T* y, bool keep, int u, int n, const typename Wide<T>::type* w, Scale s, typename Wide<T>::type per) {
     typedef typename Wide<T>::type W;
     const bool wide = a.l.bits == 8;
     const float levels = wide ? 255.0f : 15.0f;
     Unit<T> out;
     uint32_t code[2] = {0, 0};
     float q[UV<T>];
-#pragma unroll
-    for (int j = 0; j < UV<T>; j++) q[j] = quantise((double)w[j], s, per, levels);
+    quantise<UV<T>>(w, s, per, levels, q);
     if (keep) {
         if (wide) {
 #pragma unroll
@@ -299,9 +349,10 @@ template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(25
 #pragma unroll
     for (int k = 0; k < NC; k++)
 #pragma unroll
-        for (int j = 0; j < UV<T>; j++) {
+        for (int j = 0; j < UV<T>; j += 2) {   // (the end of a frame never parts a band's two values)
             w[k][j] = j < n[k] ? widen(in[k].v[j]) : W(0);
-            if (j < n[k]) range[GROUPED ? k : 0].add(w[k][j]);
+            w[k][j + 1] = j < n[k] ? widen(in[k].v[j + 1]) : W(0);
+            if (j < n[k]) range[GROUPED ? k : 0].add(w[k][j], w[k][j + 1]);
         }
     const int span = GROUPED ? 1 << a.gunits_log2 : lanes;          // lanes that hold a group
     const int start = (int)(threadIdx.x & 63) & ~(span - 1);
@@ -311,7 +362,7 @@ template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(25
         W mn = range[g].mn, mx = range[g].mx;
         for (int m = 1; m < span; m <<= 1) { mn = least(mn, __shfl_xor(mn, m)); mx = most(mx, __shfl_xor(mx, m)); }
         int flags = 0;
-        if (__ballot(!(range[g].odd == W(0))) >> start & (~0ull >> (64 - span))) {
+        if (__ballot(range[g].special()) >> start & (~0ull >> (64 - span))) {
             mn = (W)__builtin_inf(); mx = -(W)__builtin_inf();
 #pragma unroll
             for (int k = GROUPED ? g : 0; k < (GROUPED ? g + 1 : NC); k++)
@@ -320,7 +371,7 @@ template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(25
             for (int m = 1; m < span; m <<= 1) { mn = least(mn, __shfl_xor(mn, m)); mx = most(mx, __shfl_xor(mx, m)); flags |= __shfl_xor(flags, m); }
         }
         const Scale s = group_scale((double)mn, (double)mx, flags, levels);
-        const double per = reciprocal(s);
+        const W per = reciprocal(s, W(0));
         const int ug = u0 + l + g * lanes;                          // GROUPED: the unit whose group this is
         if (keep && (GROUPED ? ((ug & (span - 1)) == 0 && n[g] > 0) : l == 0))
             *(float2*)(row + a.l.scale_off + 8 * (GROUPED ? ug >> a.gunits_log2 : 0)) = make_float2(s.lo, s.step);
@@ -366,7 +417,7 @@ template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs
     __syncthreads();
     for (int i = 0; i < 4; i++) { mn = least(mn, s_mn[i]); mx = most(mx, s_mx[i]); flags |= s_flags[i]; }
     const Scale s = group_scale((double)mn, (double)mx, flags, (1 << a.l.bits) - 1);
-    const double per = reciprocal(s);
+    const W per = reciprocal(s, W(0));
     uint8_t* row = a.store + slot * a.l.row_bytes;
     T* y = a.y ? (T*)a.y + r * a.ys : nullptr;
     if (keep && t == 0) *(float2*)(row + a.l.scale_off) = make_float2(s.lo, s.step);
@@ -708,24 +759,21 @@ int cache_create(gomel_handle* h, size_t n_slots, int bits, int group_bands, gom
     c->l = l; c->device = handle_device(h); c->n_slots = n_slots;
     OnDevice dev(c->device);
     hipError_t e = dev.err;
-    const size_t bytes = n_slots * (size_t)l.row_bytes;
-    if (e == hipSuccess) e = hipMalloc((void**)&c->store, bytes);
-    if (e == hipSuccess) e = hipMalloc((void**)&c->claim, n_slots * 4);
-    if (e == hipSuccess) e = hipMalloc((void**)&c->bad, 8);
-    hipStream_t s = nullptr;   // its own: the default stream would wait for everybody's work
-    if (e == hipSuccess) e = hipStreamCreateWithFlags(&s, hipStreamNonBlocking);
-    if (e == hipSuccess) e = hipMemsetAsync(c->store, 0, bytes, s);
-    if (e == hipSuccess) e = hipMemsetAsync(c->claim, 0xFF, n_slots * 4, s);
-    if (e == hipSuccess) e = hipMemsetAsync(c->bad, 0, 8, s);
-    if (s) {
+    // one allocation: rows | claims | count of bad slots
+    const size_t rows = (n_slots * (size_t)l.row_bytes + 255) & ~(size_t)255, claims = (n_slots * 4 + 255) & ~(size_t)255;
+    if (e == hipSuccess) e = hipMalloc((void**)&c->store, rows + claims + 256);
+    if (e == hipSuccess) {
+        const hipStream_t s = handle_stream(h);   // not the default stream, which would wait for everybody's work
+        c->claim = (int32_t*)(c->store + rows);
+        c->bad = (unsigned long long*)(c->store + rows + claims);
+        e = hipMemsetAsync(c->store, 0, rows, s);
+        if (e == hipSuccess) e = hipMemsetAsync(c->claim, 0xFF, claims, s);
+        if (e == hipSuccess) e = hipMemsetAsync(c->bad, 0, 8, s);
         const hipError_t e2 = hipStreamSynchronize(s);
         if (e == hipSuccess) e = e2;
-        (void)hipStreamDestroy(s);
     }
     if (e != hipSuccess) {
         if (c->store) (void)hipFree(c->store);
-        if (c->claim) (void)hipFree(c->claim);
-        if (c->bad) (void)hipFree(c->bad);
         delete c;
         return hip_failed(e);
     }
@@ -831,7 +879,7 @@ int gomel_cache_destroy(gomel_cache* c) {
     {
         OnDevice dev(c->device);
         hipError_t e = hipDeviceSynchronize();   // calls only queue work: it may still be running on any stream
-        for (void* p : {(void*)c->store, (void*)c->claim, (void*)c->bad, c->stage}) {
+        for (void* p : {(void*)c->store, c->stage}) {
             if (!p) continue;
             const hipError_t e2 = hipFree(p);
             if (e == hipSuccess) e = e2;

@@ -11,7 +11,7 @@ struct gomel_cache {
     CacheLayout l;
     int device = 0;
     size_t n_slots = 0;
-    uint8_t* store = nullptr;           // [n_slots][row_bytes]
+    uint8_t* store = nullptr;           // [n_slots][row_bytes]; the next two lie behind it in the same allocation
     int32_t* claim = nullptr;           // [n_slots], -1 between calls: which frame of a large write gets the slot
     unsigned long long* bad = nullptr;  // frames skipped because their slot was >= n_slots
     std::mutex mu;                      // the staging buffer below
@@ -32,5 +32,6 @@ GL_HIDDEN int memory_kind(const void* p, int device);
 // defined in gomel_hip.hip
 GL_HIDDEN int handle_device(const gomel_handle* h);
 GL_HIDDEN int handle_num_mels(const gomel_handle* h);
+GL_HIDDEN hipStream_t handle_stream(const gomel_handle* h);
 GL_HIDDEN hipError_t handle_stage(gomel_handle* h, size_t bytes, void** p);   // from the handle's buffer pool
 GL_HIDDEN void handle_unstage(gomel_handle* h, void* p);

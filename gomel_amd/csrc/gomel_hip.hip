@@ -100,6 +100,7 @@ constexpr int kErrSlots = 256;
 // what the spectrogram cache and dropout (gl_cache.hip) need of a handle
 int handle_device(const gomel_handle* h) { return h->device; }
 int handle_num_mels(const gomel_handle* h) { return h->cfg.num_mels; }
+hipStream_t handle_stream(const gomel_handle* h) { return h->stream; }
 hipError_t handle_stage(gomel_handle* h, size_t bytes, void** p) { std::lock_guard<std::mutex> lk(h->mu); return (hipError_t)h->pool.alloc(p, bytes); }
 void handle_unstage(gomel_handle* h, void* p) { std::lock_guard<std::mutex> lk(h->mu); h->pool.release(p); }
 
