@@ -137,6 +137,8 @@ def _slots(slots, n, what="slots"):
     a = np.asarray(slots)
     if a.dtype.kind not in "iu" and a.size:
         raise ValueError("%s: integers are needed, not %s" % (what, a.dtype))
+    if a.dtype.kind == "u" and a.size and int(a.max()) > 2 ** 63 - 1:
+        raise ValueError("%s: beyond int64" % what)
     a = np.ascontiguousarray(a, dtype=np.int64).reshape(-1)
     if a.size != n:
         raise ValueError("%s: one slot per frame is needed (%d frames, %d slots)" % (what, n, a.size))
@@ -282,6 +284,8 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
     if out is None:
         if isinstance(x, DevicePointer):
             raise ValueError("out: a DevicePointer needs one")
+        if stream is not None and dev is not None:       # torch would hand the new tensor's memory on in the order of its own stream
+            raise ValueError("out: needed where a stream is named")
         out = np.empty(x.shape, x.dtype) if dev is None else _torch.empty(x.shape, dtype=x.dtype, device=x.device)
     optr, ot, os_, orows, ocols, odev = _flat(out, "out", write=True)
     if ot != t or getattr(out, "shape", None) != getattr(x, "shape", None) or rows * cols != orows * ocols:
@@ -311,15 +315,14 @@ def _dropout_function():
 
         class Dropout(torch.autograd.Function):
             @staticmethod
-            def forward(ctx, x, engine, p, seed, offset, stream, back):
-                ctx.args = (engine, p, seed, offset, stream, not back)
+            def forward(ctx, x, engine, p, seed, offset, back):
+                ctx.args = (engine, p, seed, offset, not back)
                 fn = _lib.lib().gomel_dropout_backward if back else _lib.lib().gomel_dropout
-                return _dropout(fn, "gomel_dropout_backward" if back else "gomel_dropout", engine, x, p, seed, offset, None, stream)
+                return _dropout(fn, "gomel_dropout_backward" if back else "gomel_dropout", engine, x, p, seed, offset, None, None)
 
             @staticmethod
             def backward(ctx, dy):
-                engine, p, seed, offset, stream, back = ctx.args
-                return Dropout.apply(dy if dy.is_contiguous() else dy.contiguous(), engine, p, seed, offset, stream, back), None, None, None, None, None, None
+                return (Dropout.apply(dy if dy.is_contiguous() else dy.contiguous(), *ctx.args),) + (None,) * 5
 
         _function = Dropout
     return _function
@@ -331,15 +334,15 @@ def _wants_grad(x):
 
 def dropout(engine, x, p, seed, offset=0, out=None, stream=None):
     if _wants_grad(x):
-        if out is not None:
-            raise ValueError("out: not with a tensor that requires a gradient")
-        return _dropout_function().apply(x, engine, p, seed, offset, stream, False)
+        if out is not None or stream is not None:
+            raise ValueError("out, stream: not with a tensor that requires a gradient")
+        return _dropout_function().apply(x, engine, p, seed, offset, False)
     return _dropout(_lib.lib().gomel_dropout, "gomel_dropout", engine, x, p, seed, offset, out, stream)
 
 
 def dropout_backward(engine, dy, p, seed, offset=0, out=None, stream=None):
     if _wants_grad(dy):
-        if out is not None:
-            raise ValueError("out: not with a tensor that requires a gradient")
-        return _dropout_function().apply(dy, engine, p, seed, offset, stream, True)
+        if out is not None or stream is not None:
+            raise ValueError("out, stream: not with a tensor that requires a gradient")
+        return _dropout_function().apply(dy, engine, p, seed, offset, True)
     return _dropout(_lib.lib().gomel_dropout_backward, "gomel_dropout_backward", engine, dy, p, seed, offset, out, stream)

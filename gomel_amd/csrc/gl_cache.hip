@@ -196,6 +196,10 @@ GL_DEV bool walk_unit(const Walk& w, int64_t* r, int64_t* u) {   // this lane's 
     return *u < w.upr;
 }
 
+// A claim as another call's kernels may be writing the same cache line right now: past this compute unit's and this die's caches.
+GL_DEV int32_t claim_of(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+GL_DEV void claim_clear(int32_t* p) { __hip_atomic_store(p, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
 struct Slots {   // where frame r goes / comes from
     const int64_t* at;
     int64_t first, n_slots;
@@ -240,7 +244,7 @@ __global__ void k_claim_clear(Slots s, int64_t n, int32_t* claim) {
     const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (r >= n) return;
     const int64_t slot = slot_of(s, r);
-    if (slot >= 0 && slot < s.n_slots) claim[slot] = -1;
+    if (slot >= 0 && slot < s.n_slots) claim_clear(claim + slot);
 }
 
 // Extremes of a group while they are being gathered.  fp32: gfx950's three-operand minimum and maximum, one instruction for two values, which
@@ -329,8 +333,8 @@ template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(25
     const int first = (int)(threadIdx.x & 63) & ~(lanes - 1);   // of this frame's lanes in the wave
     bool keep = true;
     if (a.claim) {
-        keep = a.claim[slot] == (int32_t)r;
-        if (keep && l == 0 && a.p.segs == 1) a.claim[slot] = -1;   // (a frame that lost reads its rival's index or this: neither is its own)
+        keep = claim_of(a.claim + slot) == (int32_t)r;
+        if (keep && l == 0 && a.p.segs == 1) claim_clear(a.claim + slot);   // (a frame that lost reads its rival's index or this: neither is its own)
     } else if (a.slots.at && a.n > 1) {
         bool again = false;
         for (int i = (int)r + 1 + l; i < (int)a.n; i += 8 * lanes) {   // eight loads in flight: one at a time costs 0.1 us each
@@ -395,9 +399,9 @@ template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs
     }
     bool keep = true;
     if (a.claim) {
-        keep = a.claim[slot] == (int32_t)r;
+        keep = claim_of(a.claim + slot) == (int32_t)r;
         __syncthreads();
-        if (keep && t == 0) a.claim[slot] = -1;
+        if (keep && t == 0) claim_clear(a.claim + slot);
     } else if (a.slots.at && a.n > 1) {
         int again = 0;
         for (int64_t i = r + 1 + t; i < a.n; i += 256) again |= a.slots.at[i] == slot;
@@ -715,6 +719,7 @@ int cache_call(gomel_cache* c, int type, const void* in, size_t is, void* out, s
     if (n == 0) return GOMEL_OK;
     if (n > kMaxRows || (in && !rows_span(n, cols, is)) || (out && !rows_span(n, cols, os))) return GOMEL_ERR_BAD_LENGTH;
     if (!slots && (first > c->n_slots || n > c->n_slots - first)) return GOMEL_ERR_TABLE_RANGE;
+    if ((uintptr_t)in % esz || (uintptr_t)out % esz || (uintptr_t)slots % 8) return GOMEL_ERR_BAD_CONFIG;
     if (in && out && !rows_disjoint_or_same(in, is, out, os, n, cols, esz)) return GOMEL_ERR_BAD_CONFIG;
     OnDevice dev(c->device); CHK(dev.err);
     if (vouched) { CHK(run(type, in, is, out, os, n, slots, first)); return GOMEL_OK; }
@@ -791,7 +796,7 @@ int dropout_call(gomel_handle* h, int type, const void* x, size_t xs, void* y, s
     if (rows == 0 || cols == 0) return GOMEL_OK;
     if (!x || !y) return GOMEL_ERR_NULL;
     if (!rows_span(rows, cols, xs) || !rows_span(rows, cols, ys)) return GOMEL_ERR_BAD_LENGTH;
-    if (!rows_disjoint_or_same(x, xs, y, ys, rows, cols, esz)) return GOMEL_ERR_BAD_CONFIG;
+    if ((uintptr_t)x % esz || (uintptr_t)y % esz || !rows_disjoint_or_same(x, xs, y, ys, rows, cols, esz)) return GOMEL_ERR_BAD_CONFIG;
     const int device = handle_device(h);
     OnDevice dev(device); CHK(dev.err);
     const int kx = vouched ? 1 : memory_kind(x, device), ky = vouched ? 1 : memory_kind(y, device);

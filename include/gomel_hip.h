@@ -291,8 +291,8 @@ int gomel_get_precision(const gomel_handle* h, int32_t iterations, int32_t* fp64
  * (`values`, `frames`) is left as it was.  A slot >= n_slots: in host memory the call is refused (GOMEL_ERR_TABLE_RANGE), in device
  * memory the frame is treated as padding and counted (gomel_cache_bad_slots).  The same slot twice in one write: the later frame is
  * the one that stays.
- *   `frames` and `values` are rows of 2 * NumMels elements of `type`, `stride` elements apart (>= 2 * NumMels), in host memory or
- * memory of the cache's device.  With everything in device memory a call only queues kernels on `stream` (a hipStream_t of that
+ *   `frames` and `values` are rows of 2 * NumMels elements of `type`, `stride` elements apart (>= 2 * NumMels), aligned to their
+ * element size, in host memory or memory of the cache's device.  With everything in device memory a call only queues kernels on `stream` (a hipStream_t of that
  * device; NULL = the default stream) and can be captured into a graph; with anything in host memory it copies through a staging
  * buffer and returns when it is done (not while `stream` is being captured: GOMEL_ERR_BAD_CONFIG).  Calls that touch the same
  * slots on different streams are the caller's to order.  `n` = 0 is a call without work.

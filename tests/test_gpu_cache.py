@@ -283,6 +283,29 @@ def test_a_slot_named_twice_keeps_the_last_frame(dev, n):
     e.close()
 
 
+@pytest.mark.parametrize("K,dtype,group,n", [(515, "float64", 0, 2100), (515, "float64", 32, 4200), (40, "bfloat16", 8, 6000), (1100, "float32", 0, 2048)])
+def test_a_slot_named_twice_by_claims(dev, K, dtype, group, n):
+    """The same where the frames claim their slots first: the block-wide form, frames cut into segments, many short frames.  Twice, so
+    that the claims of one call do not outlive it."""
+    e = engine(K, Resolut=8192) if K > 700 else engine(K)
+    c = e.cache(900, 8, group)
+    rng = np.random.default_rng(n)
+    base = frames(16, K, 1)
+    good = ref.stands_for(held(base, dtype), 8, group)
+    for trial in range(2):
+        which = rng.integers(0, 16, n)                       # row r holds frame which[r] of sixteen
+        slots = rng.integers(-1, 900, n).astype(np.int64)
+        c.write(dev.up(base[which], dtype), slots=dev.up(slots, "int64"))
+        got = c.read(np.empty((900, K, 2)))
+        last = {int(s): r for r, s in enumerate(slots) if s >= 0}
+        for s, r in last.items():
+            assert ref.close(got[s], (good[which[r]], np.abs(good[which[r]]) + 32), "float64", 2), (trial, s)
+        if trial == 0:
+            assert all(np.all(got[s] == 0) for s in range(900) if s not in last)
+    c.close()
+    e.close()
+
+
 def test_padding_and_bad_slots(dev):
     import gomel_amd
     K = 80
@@ -355,6 +378,11 @@ def test_refusals(dev):
     assert D(1, p, 8, p + 4, 8, 4, 8, 0.5, 0, 0, None) == 1 and D(1, p, 7, p, 8, 4, 8, 0.5, 0, 0, None) == 3
     assert D(1, None, 8, p, 8, 4, 8, 0.5, 0, 0, None) == 7
     assert D(1, None, 8, None, 8, 0, 8, 0.5, 0, 0, None) == 0
+    assert W(1, p + 2, 32, 1, None, 0, None, 0, None) == 1 and W(1, p, 32, 1, p + 4, 0, None, 0, None) == 1     # not aligned to their elements
+    assert D(1, p + 1, 8, p + 64, 8, 1, 8, 0.5, 0, 0, None) == 1
+    host = np.zeros((4, 16, 2), np.float32)
+    with pytest.raises(ValueError):
+        c.write(host, slots=np.array([0, 1, 2, 2 ** 63], np.uint64))
     c.close()
     e.close()
 
@@ -666,8 +694,8 @@ def _torch_child(rep):
     assert ref.close(c.read(np.empty((64, K, 2), np.float32), first=300), (want_of(x), np.abs(want_of(x)) + 8), "float32", 1)
 
     rep.stage("graphs")
-    for n in (32, 2500):                                 # both ways of resolving a slot named twice
-        cc = e.cache(4096, 4, 16)
+    for n in (32, 2500, 6000):                           # both ways of resolving a slot named twice
+        cc = e.cache(8192, 4, 16)
         x, slots = torch.zeros(n, K, 2, device=dev, dtype=torch.bfloat16), torch.zeros(n, dtype=torch.int64, device=dev)
         val, out, drop, back = (torch.zeros_like(x) for _ in range(4))
 
@@ -684,7 +712,7 @@ def _torch_child(rep):
                 work()
         for i in range(6):
             xi = torch.randn(n, K, 2, device=dev).to(torch.bfloat16)
-            si = torch.randperm(4096, device=dev)[:n].clone()
+            si = torch.randperm(8192, device=dev)[:n].clone()
             si[n // 2:] = si[:n - n // 2]                # slots named twice
             x.copy_(xi)
             slots.copy_(si)
@@ -728,6 +756,34 @@ def _torch_child(rep):
     with torch.no_grad():
         out = torch.empty_like(x)
         assert torch.equal(e.dropout(x, 0.3, 11, 5, out=out), y)
+    for kw in ({"stream": side}, {"out": torch.empty_like(x)}):
+        try:
+            e.dropout(x, 0.3, 11, 5, **kw)
+        except ValueError:
+            continue
+        raise AssertionError("not refused")
+    # forward and backward captured into a graph, replayed with other inputs, an eager backward between the replays
+    xs = torch.randn(64, 161, device=dev, requires_grad=True)
+    ds = torch.randn(64, 161, device=dev)
+    cap = torch.cuda.Stream()
+    cap.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(cap):
+        torch.autograd.grad(e.dropout(xs, 0.4, 3), xs, ds)
+    torch.cuda.current_stream().wait_stream(cap)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ys = e.dropout(xs, 0.4, 3)
+        (gs,) = torch.autograd.grad(ys, xs, ds)
+    for i in range(4):
+        with torch.no_grad():
+            xs.copy_(torch.randn_like(xs))
+            ds.copy_(torch.randn_like(ds))
+        g.replay()
+        torch.cuda.synchronize()
+        x2 = xs.detach().clone().requires_grad_(True)
+        y2 = e.dropout(x2, 0.4, 3)
+        (g2,) = torch.autograd.grad(y2, x2, ds)
+        assert torch.equal(ys, y2) and torch.equal(gs, g2), i
     w = torch.randn(2 * K, 64, device=dev, requires_grad=True)       # training from cached frames: cache -> dropout -> a layer -> gradients
     xin = torch.randn(128, K, 2, device=dev)
     c.write(xin, first=0)
