@@ -34,10 +34,12 @@ struct Scale { float lo, step; };
 // A finite value as fp32, the largest fp32 number standing in for what lies beyond.
 GL_DEV float to_f32(double v) { return fminf(fmaxf((float)v, -__FLT_MAX__), __FLT_MAX__); }
 
+GL_DEV float to_f32(float v) { return v; }
 // mn, mx: extremes of the group's finite values (mn > mx: there are none); flags: 1 = a NaN, 2 = a +inf, 4 = a -inf among the others.
-GL_DEV Scale group_scale(double mn, double mx, int flags, int levels) {
-    if ((flags & 1) || (mn > mx && (flags & 6) == 6)) return Scale{__builtin_nanf(""), 0.0f};
-    if (mn > mx) return Scale{(flags & 2) ? __builtin_inff() : -__builtin_inff(), 0.0f};
+template <class W> GL_DEV Scale group_scale(W mn, W mx, int flags, int levels) {
+    const bool none = mn > mx;
+    if (flags & 1 || (none && (flags & 6) == 6)) return Scale{__builtin_nanf(""), 0.0f};
+    if (none) return Scale{(flags & 2) ? __builtin_inff() : -__builtin_inff(), 0.0f};
     const float lo = to_f32(mn), hi = to_f32(mx);
     // the quotient by a constant, correctly rounded: the product with the rounded reciprocal, its remainder by multiply-add, one
     // correction (Markstein 1990); equal to the division on 4e8 pairs of fp32 numbers of every size
@@ -100,7 +102,8 @@ GL_DEV uint64_t splitmix_of(uint64_t z) {   // the word of x0's sample i (k_init
 
 // ------------------------------------------------------------------------------------------------ 16-byte units
 // A lane moves 16 bytes of frames or activations at a time: UV values of T.  Rows may start at any element (gfx950 takes a 16-byte access
-// at any element's alignment), a row's last unit may be partial.
+// at any element's alignment), a row's last unit may be partial: its first value then stands in the places behind the row's end, where
+// it changes no extreme.
 template <class T> constexpr int UV = 16 / (int)sizeof(T);
 typedef uint32_t raw_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t raw_word __attribute__((ext_vector_type(4), aligned(4)));
@@ -118,7 +121,7 @@ template <class T> struct Unit {
             __builtin_memcpy(u.v, &r, 16);
         } else {
 #pragma unroll
-            for (int j = 0; j < UV<T>; j++) u.v[j] = j < n ? p[j] : T(0.0f);
+            for (int j = 0; j < UV<T>; j++) u.v[j] = p[j < n ? j : 0];   // n >= 1
         }
         return u;
     }
@@ -253,6 +256,31 @@ GL_DEV float least(float a, float b) { asm("v_minimum3_f32 %0, %0, %1, %1" : "+v
 GL_DEV float most(float a, float b) { asm("v_maximum3_f32 %0, %0, %1, %1" : "+v"(a) : "v"(b)); return a; }
 GL_DEV double least(double a, double b) { return fmin(a, b); }
 GL_DEV double most(double a, double b) { return fmax(a, b); }
+// The value of another lane of the same 2 M neighbouring lanes, M being the power of two that was reached: the first M hold one value, the
+// other M theirs, and each gets one of the other's.  Within 16 lanes a move through the vector unit's own crossbar, no trip to LDS.
+template <int M> GL_DEV float other(float v) {
+    const int i = __builtin_bit_cast(int, v);
+    if (M == 1) return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0xB1, 0xF, 0xF, false));    // quad_perm 1,0,3,2
+    if (M == 2) return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0x4E, 0xF, 0xF, false));    // quad_perm 2,3,0,1
+    if (M == 4) return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0x141, 0xF, 0xF, false));   // row_half_mirror
+    if (M == 8) return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, 0x140, 0xF, 0xF, false));   // row_mirror
+    return __shfl_xor(v, M);
+}
+template <int M> GL_DEV double other(double v) {
+    if (M > 8) return __shfl_xor(v, M);
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const float lo = other<M>(__builtin_bit_cast(float, (uint32_t)b)), hi = other<M>(__builtin_bit_cast(float, (uint32_t)(b >> 32)));
+    return __builtin_bit_cast(double, (uint64_t)__builtin_bit_cast(uint32_t, hi) << 32 | __builtin_bit_cast(uint32_t, lo));
+}
+// Extremes over `span` neighbouring lanes (a power of two), in each of them.
+template <class W> GL_DEV void join(int span, W* mn, W* mx) {
+    if (span > 1) { *mn = least(*mn, other<1>(*mn)); *mx = most(*mx, other<1>(*mx)); }
+    if (span > 2) { *mn = least(*mn, other<2>(*mn)); *mx = most(*mx, other<2>(*mx)); }
+    if (span > 4) { *mn = least(*mn, other<4>(*mn)); *mx = most(*mx, other<4>(*mx)); }
+    if (span > 8) { *mn = least(*mn, other<8>(*mn)); *mx = most(*mx, other<8>(*mx)); }
+    if (span > 16) { *mn = least(*mn, other<16>(*mn)); *mx = most(*mx, other<16>(*mx)); }
+    if (span > 32) { *mn = least(*mn, other<32>(*mn)); *mx = most(*mx, other<32>(*mx)); }
+}
 template <class W> struct Range;
 template <> struct Range<float> {
     float mn = __builtin_inff(), mx = -__builtin_inff();
@@ -280,8 +308,26 @@ template <class W> GL_DEV void add_finite(W v, W* mn, W* mx, int* flags) {
     else { *mn = least(*mn, v); *mx = most(*mx, v); }
 }
 
-// One unit's codes into the row and, when they are asked for, its values.
-template <class T, bool S> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row, T* y, bool keep, int u, int n, const typename Wide<T>::type* w, Scale s, typename Wide<T>::type per) {
+template <int B, bool S> GL_DEV void put_code(uint8_t* p, const uint32_t* code) {   // B bytes, aligned to themselves
+    if (B == 8) {
+        typedef uint32_t two __attribute__((ext_vector_type(2)));
+        const two v = {code[0], code[B == 8]};
+        if (S) __builtin_nontemporal_store(v, (two*)p);
+        else *(two*)p = v;
+    } else if (B == 4) {
+        if (S) __builtin_nontemporal_store(code[0], (uint32_t*)p);
+        else *(uint32_t*)p = code[0];
+    } else if (B == 2) {
+        if (S) __builtin_nontemporal_store((uint16_t)code[0], (uint16_t*)p);
+        else *(uint16_t*)p = (uint16_t)code[0];
+    } else {
+        if (S) __builtin_nontemporal_store((uint8_t)code[0], p);
+        else *p = (uint8_t)code[0];
+    }
+}
+// One unit's codes into the row and, when they are asked for, its values.  S: what is stored past the caches (kStreamBytes): 1 the values,
+// 2 the codes as well.
+template <class T, int S> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row, T* y, bool keep, int u, int n, const typename Wide<T>::type* w, Scale s, typename Wide<T>::type per) {
     typedef typename Wide<T>::type W;
     const bool wide = a.l.bits == 8;
     const float levels = wide ? 255.0f : 15.0f;
@@ -292,24 +338,28 @@ template <class T, bool S> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row
     if (keep) {
         if (wide) {
 #pragma unroll
-            for (int j = 0; j < UV<T>; j++) code[j / 4] |= (uint32_t)q[j] << (8 * (j % 4));
-            __builtin_memcpy(__builtin_assume_aligned(row + u * UV<T>, UV<T>), code, UV<T>);
+            for (int j = 0; j < UV<T>; j++) code[j / 4] = __builtin_amdgcn_cvt_pk_u8_f32(q[j], j % 4, code[j / 4]);
+            put_code<UV<T>, (S > 1)>(row + u * UV<T>, code);
         } else {
 #pragma unroll
-            for (int j = 0; j < UV<T>; j++) code[0] |= (uint32_t)q[j] << (4 * j);
-            __builtin_memcpy(__builtin_assume_aligned(row + u * (UV<T> / 2), UV<T> / 2), code, UV<T> / 2);
+            for (int j = 0; j < UV<T>; j += 4) {   // four codes make a number below 2^16, exact in fp32
+                float four = q[j] + 16.0f * q[j + 1];
+                if (UV<T> > 2) four += 256.0f * (q[(j + 2) % UV<T>] + 16.0f * q[(j + 3) % UV<T>]);
+                code[0] |= (uint32_t)four << (4 * j);
+            }
+            put_code<UV<T> / 2, (S > 1)>(row + u * (UV<T> / 2), code);
         }
     }
     if (y) {
 #pragma unroll
         for (int j = 0; j < UV<T>; j++) out.v[j] = narrow<T>(dequantise(q[j], s, W(0)));
-        out.template store<S>(y + (int64_t)u * UV<T>, n);
+        out.template store<(S > 0)>(y + (int64_t)u * UV<T>, n);
     }
 }
 
 // A frame -- or, of a wide grouped one, a segment of it -- lies in the registers of its lanes (Spread).  Its extremes are joined across
 // those lanes (a group's across the lanes of the group), the codes follow from the same registers: the frames are read once.
-template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(256) void k_write(WriteArgs a) {
+template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256) void k_write(WriteArgs a) {
     typedef typename Wide<T>::type W;
     const int lanes = 1 << a.p.lanes_log2, l = (int)threadIdx.x & (lanes - 1);
     const int64_t part = (int64_t)blockIdx.x * (256 >> a.p.lanes_log2) + ((int)threadIdx.x >> a.p.lanes_log2);
@@ -323,7 +373,7 @@ template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(25
     for (int k = 0; k < NC; k++) {
         const int c = (u0 + l + k * lanes) * UV<T>;
         n[k] = min(UV<T>, 2 * a.l.K - c);
-        if (n[k] > 0) in[k] = Unit<T>::template load<S>(x + c, n[k]);
+        if (n[k] > 0) in[k] = Unit<T>::template load<(S > 0)>(x + c, n[k]);
     }
     const int64_t slot = slot_of(a.slots, r);
     if (slot < 0 || slot >= a.slots.n_slots) {
@@ -351,30 +401,31 @@ template <class T, int NC, bool GROUPED, bool S> __global__ __launch_bounds__(25
     W w[NC][UV<T>];
     Range<W> range[GROUPED ? NC : 1];
 #pragma unroll
-    for (int k = 0; k < NC; k++)
+    for (int k = 0; k < NC; k++) {
+        if (n[k] <= 0) continue;
 #pragma unroll
-        for (int j = 0; j < UV<T>; j += 2) {   // (the end of a frame never parts a band's two values)
-            w[k][j] = j < n[k] ? widen(in[k].v[j]) : W(0);
-            w[k][j + 1] = j < n[k] ? widen(in[k].v[j + 1]) : W(0);
-            if (j < n[k]) range[GROUPED ? k : 0].add(w[k][j], w[k][j + 1]);
-        }
+        for (int j = 0; j < UV<T>; j++) w[k][j] = widen(in[k].v[j]);
+#pragma unroll
+        for (int j = 0; j < UV<T>; j += 2) range[GROUPED ? k : 0].add(w[k][j], w[k][j + 1]);
+    }
     const int span = GROUPED ? 1 << a.gunits_log2 : lanes;          // lanes that hold a group
     const int start = (int)(threadIdx.x & 63) & ~(span - 1);
     const int levels = (1 << a.l.bits) - 1;
 #pragma unroll
     for (int g = 0; g < (GROUPED ? NC : 1); g++) {
         W mn = range[g].mn, mx = range[g].mx;
-        for (int m = 1; m < span; m <<= 1) { mn = least(mn, __shfl_xor(mn, m)); mx = most(mx, __shfl_xor(mx, m)); }
+        join(span, &mn, &mx);
         int flags = 0;
         if (__ballot(range[g].special()) >> start & (~0ull >> (64 - span))) {
             mn = (W)__builtin_inf(); mx = -(W)__builtin_inf();
 #pragma unroll
             for (int k = GROUPED ? g : 0; k < (GROUPED ? g + 1 : NC); k++)
 #pragma unroll
-                for (int j = 0; j < UV<T>; j++) if (j < n[k]) add_finite(w[k][j], &mn, &mx, &flags);
-            for (int m = 1; m < span; m <<= 1) { mn = least(mn, __shfl_xor(mn, m)); mx = most(mx, __shfl_xor(mx, m)); flags |= __shfl_xor(flags, m); }
+                for (int j = 0; j < UV<T>; j++) if (n[k] > 0) add_finite(w[k][j], &mn, &mx, &flags);
+            join(span, &mn, &mx);
+            for (int m = 1; m < span; m <<= 1) flags |= __shfl_xor(flags, m);
         }
-        const Scale s = group_scale((double)mn, (double)mx, flags, levels);
+        const Scale s = group_scale(mn, mx, flags, levels);
         const W per = reciprocal(s, W(0));
         const int ug = u0 + l + g * lanes;                          // GROUPED: the unit whose group this is
         if (keep && (GROUPED ? ((ug & (span - 1)) == 0 && n[g] > 0) : l == 0))
@@ -414,13 +465,14 @@ template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs
         const int n = min(UV<T>, cols - c);
         const Unit<T> in = Unit<T>::template load<false>(x + c, n);
 #pragma unroll
-        for (int j = 0; j < UV<T>; j++) if (j < n) add_finite(widen(in.v[j]), &mn, &mx, &flags);
+        for (int j = 0; j < UV<T>; j++) add_finite(widen(in.v[j]), &mn, &mx, &flags);
     }
-    for (int m = 1; m < 64; m <<= 1) { mn = least(mn, __shfl_xor(mn, m)); mx = most(mx, __shfl_xor(mx, m)); flags |= __shfl_xor(flags, m); }
+    join(64, &mn, &mx);
+    for (int m = 1; m < 64; m <<= 1) flags |= __shfl_xor(flags, m);
     if ((t & 63) == 0) { s_mn[t >> 6] = mn; s_mx[t >> 6] = mx; s_flags[t >> 6] = flags; }
     __syncthreads();
     for (int i = 0; i < 4; i++) { mn = least(mn, s_mn[i]); mx = most(mx, s_mx[i]); flags |= s_flags[i]; }
-    const Scale s = group_scale((double)mn, (double)mx, flags, (1 << a.l.bits) - 1);
+    const Scale s = group_scale(mn, mx, flags, (1 << a.l.bits) - 1);
     const W per = reciprocal(s, W(0));
     uint8_t* row = a.store + slot * a.l.row_bytes;
     T* y = a.y ? (T*)a.y + r * a.ys : nullptr;
@@ -430,8 +482,8 @@ template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs
         const Unit<T> in = Unit<T>::template load<false>(x + c, n);
         W w[UV<T>];
 #pragma unroll
-        for (int j = 0; j < UV<T>; j++) w[j] = j < n ? widen(in.v[j]) : W(0);
-        put_unit<T, false>(a, row, y, keep, c / UV<T>, n, w, s, per);
+        for (int j = 0; j < UV<T>; j++) w[j] = widen(in.v[j]);
+        put_unit<T, 0>(a, row, y, keep, c / UV<T>, n, w, s, per);
     }
 }
 
@@ -594,7 +646,7 @@ template <class T, bool S> __global__ __launch_bounds__(512) void k_dropout_rows
         case GOMEL_F16: { typedef __half T; __VA_ARGS__; } break;    \
         default: { typedef __hip_bfloat16 T; __VA_ARGS__; } break;   \
     }
-template <class T, bool G, bool S> void (*write_kernel(int units))(WriteArgs) {
+template <class T, bool G, int S> void (*write_kernel(int units))(WriteArgs) {
     switch (units) {
         case 1: return k_write<T, 1, G, S>;
         case 2: return k_write<T, 2, G, S>;
@@ -604,9 +656,9 @@ template <class T, bool G, bool S> void (*write_kernel(int units))(WriteArgs) {
         default: return k_write<T, 6, G, S>;
     }
 }
-template <class T> void (*write_kernel(int units, bool grouped, bool streamed))(WriteArgs) {
-    if (grouped) return streamed ? write_kernel<T, true, true>(units) : write_kernel<T, true, false>(units);
-    return streamed ? write_kernel<T, false, true>(units) : write_kernel<T, false, false>(units);
+template <class T> void (*write_kernel(int units, bool grouped, int streamed))(WriteArgs) {
+    if (grouped) return streamed == 2 ? write_kernel<T, true, 2>(units) : streamed ? write_kernel<T, true, 1>(units) : write_kernel<T, true, 0>(units);
+    return streamed == 2 ? write_kernel<T, false, 2>(units) : streamed ? write_kernel<T, false, 1>(units) : write_kernel<T, false, 0>(units);
 }
 template <class T, int BITS, bool S> void (*read_kernel(int units, bool dropping))(ReadArgs) {
     if (dropping) return k_read_drop<T, BITS, S>;
@@ -852,7 +904,8 @@ hipError_t cache_write_device(gomel_cache* c, int type, const void* x, size_t xs
     }
     const size_t per = 256 >> a.p.lanes_log2, blocks = (n * (size_t)a.p.segs + per - 1) / per;
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    GL_TYPES(type, e = launch(write_kernel<T>(a.p.units, grouped, 2 * (size_t)c->l.K * n * type_bytes(type) >= kStreamBytes), (unsigned)blocks, 256, s, a));
+    const int streamed = 2 * (size_t)c->l.K * n * type_bytes(type) < kStreamBytes ? 0 : n * (size_t)c->l.row_bytes < kStreamInBytes ? 1 : 2;
+    GL_TYPES(type, e = launch(write_kernel<T>(a.p.units, grouped, streamed), (unsigned)blocks, 256, s, a));
     if (claims && a.p.segs > 1 && e == hipSuccess) e = launch_claim(k_claim_clear, a.slots, a.n, c->claim, s);
     return e;
 }
