@@ -199,9 +199,10 @@ GL_DEV bool walk_unit(const Walk& w, int64_t* r, int64_t* u) {   // this lane's 
     return *u < w.upr;
 }
 
-// A claim as another call's kernels may be writing the same cache line right now: past this compute unit's and this die's caches.
+// A claim is read past this compute unit's and this die's caches: a call on another stream may be claiming neighbouring slots (the same
+// cache line) right now, and a line kept from before that would show this call's claims as they were then.  The -1 that takes a claim
+// back is an ordinary store: it is written back, by its own bytes, before the next kernel of the stream starts.
 GL_DEV int32_t claim_of(const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-GL_DEV void claim_clear(int32_t* p) { __hip_atomic_store(p, -1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 struct Slots {   // where frame r goes / comes from
     const int64_t* at;
@@ -247,7 +248,7 @@ __global__ void k_claim_clear(Slots s, int64_t n, int32_t* claim) {
     const int64_t r = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (r >= n) return;
     const int64_t slot = slot_of(s, r);
-    if (slot >= 0 && slot < s.n_slots) claim_clear(claim + slot);
+    if (slot >= 0 && slot < s.n_slots) claim[slot] = -1;
 }
 
 // Extremes of a group while they are being gathered.  fp32: gfx950's three-operand minimum and maximum, one instruction for two values, which
@@ -366,6 +367,7 @@ template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256
     if (part >= a.n * a.p.segs) return;
     const int64_t r = a.p.segs == 1 ? part : part / a.p.segs;
     const int u0 = a.p.segs == 1 ? 0 : (int)(part - r * a.p.segs) * (NC * lanes);
+    const int64_t slot = slot_of(a.slots, r);   // before the frame's loads: the claim hangs on it and comes while they are on their way
     const T* x = (const T*)a.x + r * a.xs;
     Unit<T> in[NC];
     int n[NC];
@@ -375,17 +377,14 @@ template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256
         n[k] = min(UV<T>, 2 * a.l.K - c);
         if (n[k] > 0) in[k] = Unit<T>::template load<(S > 0)>(x + c, n[k]);
     }
-    const int64_t slot = slot_of(a.slots, r);
     if (slot < 0 || slot >= a.slots.n_slots) {
         if (slot >= a.slots.n_slots && l == 0 && u0 == 0) atomicAdd(a.bad, 1ull);
         return;
     }
     const int first = (int)(threadIdx.x & 63) & ~(lanes - 1);   // of this frame's lanes in the wave
-    bool keep = true;
-    if (a.claim) {
-        keep = claim_of(a.claim + slot) == (int32_t)r;
-        if (keep && l == 0 && a.p.segs == 1) claim_clear(a.claim + slot);   // (a frame that lost reads its rival's index or this: neither is its own)
-    } else if (a.slots.at && a.n > 1) {
+    int32_t owner = (int32_t)r;
+    if (a.claim) owner = claim_of(a.claim + slot);
+    else if (a.slots.at && a.n > 1) {
         bool again = false;
         for (int i = (int)r + 1 + l; i < (int)a.n; i += 8 * lanes) {   // eight loads in flight: one at a time costs 0.1 us each
             int64_t at[8];
@@ -394,7 +393,7 @@ template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256
 #pragma unroll
             for (int k = 0; k < 8; k++) again |= at[k] == slot && i + k * lanes < (int)a.n;
         }
-        keep = !(__ballot(again) >> first & (~0ull >> (64 - lanes)));
+        if (__ballot(again) >> first & (~0ull >> (64 - lanes))) owner = -1;
     }
     uint8_t* row = a.store + slot * a.l.row_bytes;
     T* y = a.y ? (T*)a.y + r * a.ys : nullptr;
@@ -408,6 +407,7 @@ template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256
 #pragma unroll
         for (int j = 0; j < UV<T>; j += 2) range[GROUPED ? k : 0].add(w[k][j], w[k][j + 1]);
     }
+    const bool keep = owner == (int32_t)r;
     const int span = GROUPED ? 1 << a.gunits_log2 : lanes;          // lanes that hold a group
     const int start = (int)(threadIdx.x & 63) & ~(span - 1);
     const int levels = (1 << a.l.bits) - 1;
@@ -434,6 +434,7 @@ template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256
         for (int k = GROUPED ? g : 0; k < (GROUPED ? g + 1 : NC); k++)
             if (n[k] > 0) put_unit<T, S>(a, row, y, keep, u0 + l + k * lanes, n[k], w[k], s, per);
     }
+    if (a.claim && keep && l == 0 && a.p.segs == 1) a.claim[slot] = -1;   // (a frame that lost reads its rival's index or this: neither is its own)
 }
 
 // A frame under one scale that is too wide for a wave's registers: a block per frame, which reads it twice (the second time out of the
@@ -452,7 +453,7 @@ template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs
     if (a.claim) {
         keep = claim_of(a.claim + slot) == (int32_t)r;
         __syncthreads();
-        if (keep && t == 0) claim_clear(a.claim + slot);
+        if (keep && t == 0) a.claim[slot] = -1;
     } else if (a.slots.at && a.n > 1) {
         int again = 0;
         for (int64_t i = r + 1 + t; i < a.n; i += 256) again |= a.slots.at[i] == slot;
