@@ -36,41 +36,47 @@ def needs_build(out=OUT):
     return any(os.path.exists(d) and os.path.getmtime(d) > t for d in DEPS)
 
 
+def _report(stderr):
+    err = "\n".join(l for l in stderr.splitlines() if "is not a recognized feature for this target" not in l)
+    if err.strip():
+        print(err, file=sys.stderr)
+
+
 def _run(cmd, verbose):
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     r = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
-    err = "\n".join(l for l in r.stderr.splitlines() if "is not a recognized feature for this target" not in l)
-    if err.strip():
-        print(err, file=sys.stderr)
+    _report(r.stderr)
     if r.returncode:
         raise subprocess.CalledProcessError(r.returncode, cmd)
 
 
 def build(force=False, verbose=False, out=OUT, extra_flags=()):
-    """Compile every source into `out` (default gomel_amd/libgomel_hip.so).  extra_flags: -D knobs of an A/B build (both
-    translation units get them).  Returns the path."""
+    """Compile every source into `out` (default gomel_amd/libgomel_hip.so).  extra_flags: -D knobs of an A/B build (every
+    translation unit gets them).  Returns the path."""
     if not force and not extra_flags and not needs_build(out):
         return out
     with tempfile.TemporaryDirectory(prefix="gomel_build_") as tmp:
         host_o, hip_o, cache_o = (os.path.join(tmp, n) for n in ("gomel_host.o", "gomel_hip.o", "gl_cache.o"))
         cxx = shutil.which("g++") or shutil.which("c++")
         host_cmd = ([cxx] if cxx else [hipcc(), "-x", "c++"]) + HOST_FLAGS + list(extra_flags) + ["-c", HOST_SRC, "-o", host_o]   # (no g++: the host pass of hipcc's clang)
-        if verbose:
-            print(" ".join(host_cmd), file=sys.stderr)
-        host = subprocess.Popen(host_cmd, stderr=subprocess.PIPE, text=True)                 # beside the device compile
+        cache_cmd = [hipcc()] + CACHE_FLAGS + list(extra_flags) + ["-c", CACHE_SRC, "-o", cache_o]
+        beside = []                        # the smaller compiles run beside the Griffin-Lim kernels'
         try:
-            _run([hipcc()] + CACHE_FLAGS + list(extra_flags) + ["-c", CACHE_SRC, "-o", cache_o], verbose)
+            for cmd in (host_cmd, cache_cmd):
+                if verbose:
+                    print(" ".join(cmd), file=sys.stderr)
+                beside.append((cmd, subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True)))
             _run([hipcc()] + HIP_FLAGS + list(extra_flags) + ["-c", SRC, "-o", hip_o], verbose)
-            _, host_err = host.communicate()
-            if host_err.strip():
-                print(host_err, file=sys.stderr)
-            if host.returncode:
-                raise subprocess.CalledProcessError(host.returncode, host_cmd)
+            for cmd, child in beside:
+                _report(child.communicate()[1])
+                if child.returncode:
+                    raise subprocess.CalledProcessError(child.returncode, cmd)
         finally:
-            if host.poll() is None:        # the device compile failed: do not leave the host compile writing into a directory that is about to go
-                host.kill()
-                host.communicate()
+            for _, child in beside:
+                if child.poll() is None:   # another compile failed: do not leave this one writing into a directory that is about to go
+                    child.kill()
+                    child.communicate()
         _run([hipcc(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", out + ".tmp", hip_o, cache_o, host_o], verbose)
     os.replace(out + ".tmp", out)
     return out
