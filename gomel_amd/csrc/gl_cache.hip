@@ -33,7 +33,6 @@ struct Scale { float lo, step; };
 
 // A finite value as fp32, the largest fp32 number standing in for what lies beyond.
 GL_DEV float to_f32(double v) { return fminf(fmaxf((float)v, -__FLT_MAX__), __FLT_MAX__); }
-
 GL_DEV float to_f32(float v) { return v; }
 // mn, mx: extremes of the group's finite values (mn > mx: there are none); flags: 1 = a NaN, 2 = a +inf, 4 = a -inf among the others.
 template <class W> GL_DEV Scale group_scale(W mn, W mx, int flags, int levels) {
@@ -53,10 +52,11 @@ GL_DEV float code_of(double v, Scale s, float levels) {
     return fminf(fmaxf((float)rint((v - (double)s.lo) / (double)s.step), 0.0f), levels);
 }
 // The codes of N values at once.  The quotients come from products with 1 / step first, and a value whose product is so near a border that
-// the rounding of difference, reciprocal and product could have carried it across -- `margin` -- sends the lane to the definition.
+// the rounding of difference, reciprocal and product could have carried it across sends the lane to the definition.
 //   fp32 (and the 16-bit types): v - lo is off by 2^-24 of itself, v_rcp_f32 by 2^-23, the product by 2^-24: 2^-22 of a quotient of at
-// most `levels` (and a little), so levels * 2^-21 is twice what is needed; one value in 4000 is that near at 8 bits.  fp32 instructions
-// cost what fp64 ones do here, but the definition's take twice as many: a 16-bit write was bound by them.
+// most `levels` (and a little), so levels * 2^-21 is twice what is needed; one value in 4000 is that near at 8 bits.  Instructions of
+// either width cost the same here, but the definition takes twice as many: a write of 16-bit frames was bound by them (192 bands: 740
+// vector instructions per wave and 193 us for 409 600 frames with values, now 400 and 174).
 //   fp64: 2^-51 of the quotient; 2^-33 is far beyond it and as rare as never.
 // Whatever is not a number in between (an infinite value, a step whose reciprocal fp32 does not hold) fails the comparison and goes there too.
 template <int N> GL_DEV void quantise(const float* v, Scale s, float per, float levels, float* q) {
@@ -185,17 +185,17 @@ inline Walk walk_of(size_t rows, size_t upr) {
     }
     return w;
 }
-GL_DEV bool walk_unit(const Walk& w, int64_t* r, int64_t* u) {   // this lane's unit; false: there is none
+GL_DEV bool walk_unit(const Walk& w, int64_t block, int64_t* r, int64_t* u) {   // this lane's unit; false: there is none
     const int i = (int)threadIdx.x;
     if (w.rpb) {
         const uint32_t q = w.upr == 1 ? (uint32_t)i : (uint32_t)(((uint64_t)(uint32_t)i * w.magic) >> 32);
-        *r = (int64_t)blockIdx.x * w.rpb + q;
+        *r = block * w.rpb + q;
         *u = i - (int64_t)q * w.upr;
         return (int)q < w.rpb && *r < w.rows;
     }
-    const int64_t b = (int64_t)blockIdx.x / w.segs;
+    const int64_t b = block / w.segs;
     *r = b;
-    *u = ((int64_t)blockIdx.x - b * w.segs) * w.block + i;
+    *u = (block - b * w.segs) * w.block + i;
     return *u < w.upr;
 }
 
@@ -220,6 +220,7 @@ struct WriteArgs {
     unsigned long long* bad;
     Spread p;
     int32_t gunits_log2;      // a group's units
+    int64_t block0 = 0;
 };
 struct ReadArgs {
     void* y;
@@ -233,6 +234,7 @@ struct ReadArgs {
     uint64_t seed, offset;
     unsigned long long* bad;
     int32_t wraps;            // offset + the output's elements pass 2^64
+    int64_t block0 = 0;
 };
 
 // Which frame keeps a slot that a write names more than once: the last.  The rows of a call claim their slots with an atomic maximum
@@ -363,7 +365,7 @@ template <class T, int S> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row,
 template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256) void k_write(WriteArgs a) {
     typedef typename Wide<T>::type W;
     const int lanes = 1 << a.p.lanes_log2, l = (int)threadIdx.x & (lanes - 1);
-    const int64_t part = (int64_t)blockIdx.x * (256 >> a.p.lanes_log2) + ((int)threadIdx.x >> a.p.lanes_log2);
+    const int64_t part = (a.block0 + blockIdx.x) * (256 >> a.p.lanes_log2) + ((int)threadIdx.x >> a.p.lanes_log2);
     if (part >= a.n * a.p.segs) return;
     const int64_t r = a.p.segs == 1 ? part : part / a.p.segs;
     const int u0 = a.p.segs == 1 ? 0 : (int)(part - r * a.p.segs) * (NC * lanes);
@@ -443,7 +445,7 @@ template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs
     typedef typename Wide<T>::type W;
     __shared__ W s_mn[4], s_mx[4];
     __shared__ int s_flags[4];
-    const int64_t r = blockIdx.x, slot = slot_of(a.slots, r);
+    const int64_t r = a.block0 + blockIdx.x, slot = slot_of(a.slots, r);
     const int t = (int)threadIdx.x, cols = 2 * a.l.K;
     if (slot < 0 || slot >= a.slots.n_slots) {
         if (slot >= a.slots.n_slots && t == 0) atomicAdd(a.bad, 1ull);
@@ -521,7 +523,7 @@ template <class T> GL_DEV T drop_or(typename Wide<T>::type v, const DropRule& d,
 // What k_read and k_read_drop share: the frame this lane works on, its first unit there, the frame's row in the cache; false: none.
 GL_DEV bool read_place(const ReadArgs& a, int units, int64_t* r, int* u0, const uint8_t** row) {
     const int lanes = 1 << a.p.lanes_log2, l = (int)threadIdx.x & (lanes - 1);
-    const int64_t part = (int64_t)blockIdx.x * (256 >> a.p.lanes_log2) + ((int)threadIdx.x >> a.p.lanes_log2);
+    const int64_t part = (a.block0 + blockIdx.x) * (256 >> a.p.lanes_log2) + ((int)threadIdx.x >> a.p.lanes_log2);
     if (part >= a.n * a.p.segs) return false;
     *r = a.p.segs == 1 ? part : part / a.p.segs;
     *u0 = (a.p.segs == 1 ? 0 : (int)(part - *r * a.p.segs) * (units * lanes)) + l;
@@ -609,12 +611,13 @@ struct DropArgs {
     DropRule drop;
     uint64_t seed, offset;
     int32_t wraps;            // offset + total pass 2^64
+    int64_t block0 = 0;
 };
 // Dense arrays: one unit per lane.  Bound by HBM in fp32 and fp64 (two streams), by the generator's multiplications in the 16-bit types:
 // six quarter-rate 32-bit products for two elements.  One unit per lane is the best of 1, 2, 4 and 8: with more in flight per lane
 // fp32 falls from 6.17 to 5.9 TB/s, bf16 from 6.08 to 5.8 (409 600 x 384 elements, bytes read and written).
 template <class T, bool S, bool LN> __global__ __launch_bounds__(256) void k_dropout(DropArgs a) {
-    const int64_t e0 = (int64_t)blockIdx.x * (256 * UV<T>);
+    const int64_t e0 = (a.block0 + blockIdx.x) * (256 * UV<T>);
     const int t = (int)threadIdx.x * UV<T>;
     const int n = (int)min((int64_t)UV<T>, a.total - e0 - t);
     if (n <= 0) return;
@@ -628,7 +631,7 @@ template <class T, bool S, bool LN> __global__ __launch_bounds__(256) void k_dro
 // Rows apart.
 template <class T, bool S> __global__ __launch_bounds__(512) void k_dropout_rows(DropArgs a) {
     int64_t r, k;
-    if (!walk_unit(a.w, &r, &k)) return;
+    if (!walk_unit(a.w, a.block0 + blockIdx.x, &r, &k)) return;
     const int64_t c = k * UV<T>;
     const int n = (int)min((int64_t)UV<T>, a.cols - c);
     Unit<T> x = Unit<T>::template load<false>((const T*)a.x + r * a.xs + c, n);
@@ -683,10 +686,17 @@ template <class T> void (*read_kernel(int bits, int units, bool dropping, bool s
 // quarter of that cache nothing is gained.  Frames to be written are loaded so too, dropout's input where input and output together do
 // not fit (315 MB of fp32: 194.9 instead of 199.2 us; 79 MB: 26.7 instead of 23.8).
 constexpr size_t kStreamBytes = (size_t)64 << 20, kStreamInBytes = (size_t)128 << 20;
-// launches report their own status: hipGetLastError could hand back somebody else's
-template <class Args> hipError_t launch(void (*k)(Args), unsigned grid, unsigned block, hipStream_t s, Args& a) {
-    void* p[] = {&a};
-    return hipLaunchKernel((const void*)k, dim3(grid), dim3(block), p, 0, s);
+// A launch has fewer than 2^32 lanes: grids of more blocks go out in parts, a block's index counted on through them (`block0`).  Launches
+// report their own status: hipGetLastError could hand back somebody else's.
+constexpr size_t kBlocks = (size_t)1 << 22;
+template <class Args> hipError_t launch(void (*k)(Args), size_t blocks, unsigned block, hipStream_t s, Args& a) {
+    hipError_t e = hipSuccess;
+    for (size_t b = 0; b < blocks && e == hipSuccess; b += kBlocks) {
+        a.block0 = (int64_t)b;
+        void* p[] = {&a};
+        e = hipLaunchKernel((const void*)k, dim3((unsigned)std::min(kBlocks, blocks - b)), dim3(block), p, 0, s);
+    }
+    return e;
 }
 hipError_t launch_claim(void (*k)(Slots, int64_t, int32_t*), Slots sl, int64_t n, int32_t* claim, hipStream_t s) {
     void* p[] = {&sl, &n, &claim};
@@ -719,14 +729,12 @@ hipError_t dropout_device(int type, const void* x, size_t xs, void* y, size_t ys
     hipError_t e = hipSuccess;
     if ((xs == cols && ys == cols) || rows == 1) {
         const size_t units = (total + uv - 1) / uv, blocks = (units + 256 - 1) / 256;
-        if (blocks > INT32_MAX) return hipErrorInvalidValue;
         GL_TYPES(type, e = launch(bytes < kStreamBytes ? k_dropout<T, false, false> : bytes < kStreamInBytes ? k_dropout<T, true, false> : k_dropout<T, true, true>,
-                                  (unsigned)blocks, 256, s, a));
+                                  blocks, 256, s, a));
         return e;
     }
     a.w = walk_of(rows, (cols + uv - 1) / uv);
-    if (a.w.blocks > INT32_MAX) return hipErrorInvalidValue;
-    GL_TYPES(type, e = launch(bytes < kStreamBytes ? k_dropout_rows<T, false> : k_dropout_rows<T, true>, (unsigned)a.w.blocks, (unsigned)a.w.block, s, a));
+    GL_TYPES(type, e = launch(bytes < kStreamBytes ? k_dropout_rows<T, false> : k_dropout_rows<T, true>, (size_t)a.w.blocks, (unsigned)a.w.block, s, a));
     return e;
 }
 
@@ -737,12 +745,12 @@ constexpr size_t kScanPerLane = 64;
 
 // Rows between host memory (stride elements apart) and a dense device buffer
 hipError_t rows_in(void* dev, const char* host, size_t stride, size_t rows, size_t cols, size_t esz, hipStream_t s) {
-    if (stride == cols || rows == 1) return hipMemcpyAsync(dev, host, rows * cols * esz, hipMemcpyHostToDevice, s);
-    return hipMemcpy2DAsync(dev, cols * esz, host, stride * esz, cols * esz, rows, hipMemcpyHostToDevice, s);
+    if (stride == cols || rows == 1) return hipMemcpyAsync(dev, host, rows * cols * esz, hipMemcpyDefault, s);
+    return hipMemcpy2DAsync(dev, cols * esz, host, stride * esz, cols * esz, rows, hipMemcpyDefault, s);
 }
 hipError_t rows_out(char* host, const void* dev, size_t stride, size_t rows, size_t cols, size_t esz, hipStream_t s) {
-    if (stride == cols || rows == 1) return hipMemcpyAsync(host, dev, rows * cols * esz, hipMemcpyDeviceToHost, s);
-    return hipMemcpy2DAsync(host, stride * esz, dev, cols * esz, cols * esz, rows, hipMemcpyDeviceToHost, s);
+    if (stride == cols || rows == 1) return hipMemcpyAsync(host, dev, rows * cols * esz, hipMemcpyDefault, s);
+    return hipMemcpy2DAsync(host, stride * esz, dev, cols * esz, cols * esz, rows, hipMemcpyDefault, s);
 }
 
 int cache_stage(gomel_cache* c, size_t bytes, char** p) {   // caller holds c->mu
@@ -794,7 +802,7 @@ int cache_call(gomel_cache* c, int type, const void* in, size_t is, void* out, s
         const char* from = in ? (const char*)in + r * is * esz : nullptr;
         char* to = out ? (char*)out + r * os * esz : nullptr;
         const int64_t* at = slots ? slots + r : nullptr;
-        if (!ks) e = hipMemcpyAsync(st_slots, at, m * 8, hipMemcpyHostToDevice, s);
+        if (!ks) e = hipMemcpyAsync(st_slots, at, m * 8, hipMemcpyDefault, s);
         if (!ki && e == hipSuccess) e = rows_in(st, from, is, m, cols, esz, s);
         if (!ko && slots && e == hipSuccess) e = rows_in(st_out, to, os, m, cols, esz, s);   // rows of padding come back as they were
         if (e == hipSuccess) e = run(type, ki ? from : st, ki ? is : cols, ko ? to : st_out, ko ? os : cols, m, ks ? at : (const int64_t*)st_slots, first + r);
@@ -900,13 +908,12 @@ hipError_t cache_write_device(gomel_cache* c, int type, const void* x, size_t xs
     if (claims) e = launch_claim(k_claim, a.slots, a.n, c->claim, s);
     if (e != hipSuccess) return e;
     if (!a.p.units) {
-        GL_TYPES(type, e = launch(k_write_wide<T>, (unsigned)n, 256, s, a));
+        GL_TYPES(type, e = launch(k_write_wide<T>, n, 256, s, a));
         return e;
     }
     const size_t per = 256 >> a.p.lanes_log2, blocks = (n * (size_t)a.p.segs + per - 1) / per;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
     const int streamed = 2 * (size_t)c->l.K * n * type_bytes(type) < kStreamBytes ? 0 : n * (size_t)c->l.row_bytes < kStreamInBytes ? 1 : 2;
-    GL_TYPES(type, e = launch(write_kernel<T>(a.p.units, grouped, streamed), (unsigned)blocks, 256, s, a));
+    GL_TYPES(type, e = launch(write_kernel<T>(a.p.units, grouped, streamed), blocks, 256, s, a));
     if (claims && a.p.segs > 1 && e == hipSuccess) e = launch_claim(k_claim_clear, a.slots, a.n, c->claim, s);
     return e;
 }
@@ -919,10 +926,9 @@ hipError_t cache_read_device(gomel_cache* c, int type, void* y, size_t ys, size_
     ReadArgs a{y, (int64_t)ys, (int64_t)n, Slots{slots, (int64_t)first, (int64_t)c->n_slots}, c->store, c->l, spread_of(n, (2 * c->l.K + uv - 1) / uv, 3, true), drop,
                gshift, (int32_t)strict, seed, offset, bad ? bad : c->bad, (int32_t)(offset + 2 * (uint64_t)c->l.K * n < offset)};
     const size_t per = 256 >> a.p.lanes_log2, blocks = (n * (size_t)a.p.segs + per - 1) / per;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    const bool dropping = drop.all || drop.below != 0;
+    const bool dropping = drop.all || drop.below != 0 || drop.scale != 1.0;   // (p below 2^-33 drops nothing, its factor stays)
     hipError_t e = hipSuccess;
-    GL_TYPES(type, e = launch(read_kernel<T>(c->l.bits, a.p.units, dropping, 2 * (size_t)c->l.K * n * type_bytes(type) >= kStreamBytes), (unsigned)blocks, 256, s, a));
+    GL_TYPES(type, e = launch(read_kernel<T>(c->l.bits, a.p.units, dropping, 2 * (size_t)c->l.K * n * type_bytes(type) >= kStreamBytes), blocks, 256, s, a));
     return e;
 }
 

@@ -313,7 +313,7 @@ int gomel_cache_read(gomel_cache* c, int type, void* frames, size_t stride, size
 /* How many frames were skipped so far because their slot, in device memory, was >= n_slots; counts the calls whose work has finished
  * (synchronise their streams first) and starts again at zero. */
 int gomel_cache_bad_slots(gomel_cache* c, uint64_t* count);
-/* gomel_batch_upload with the spectrograms taken from a cache of the same NumMels and device: slots[f] for the batch's frames in
+/* gomel_batch_upload (of a batch of gomel_batch_create) with the spectrograms taken from a cache of the same NumMels and device: slots[f] for the batch's frames in
  * order (host or device memory; every one a slot of the cache: padding and slots >= n_slots are refused with GOMEL_ERR_TABLE_RANGE,
  * and the batch then has to be uploaded again).  Work queued on `stream` before the call is seen.  Returns when the batch is uploaded,
  * as gomel_batch_upload does. */

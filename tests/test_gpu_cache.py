@@ -489,6 +489,27 @@ def test_dropout_beyond_32_bit_indexes(dev):
     e.close()
 
 
+def test_more_frames_than_one_launch_takes(dev):
+    """200 million one-band frames (the grids go out in parts): dropout, write and read reach the first, the last and those at the seams."""
+    e = engine(1)
+    n = 200_000_003
+    c = e.cache(n, 8, 0)
+    x, y = dev.empty(2 * n, "float16"), dev.empty(2 * n, "float16")
+    assert dev.hip.hipMemset(x.data_ptr(), 0x3C, 4 * n) == 0                    # 0x3C3C = 1.05859375
+    e.dropout(x, 0.5, 33, 0, out=x)
+    c.write(x)
+    c.read(y)
+    seam = (1 << 22) * 32                                                      # blocks of a launch x frames of a block (8 lanes each)
+    for at in (0, seam - 500, n - 1000, 2 * (1 << 22) * 8 - 700):
+        want = np.where(ref.dropped(0.5, 33, 2 * at, 2000), 0, 2.1171875)
+        for d in (x, y):
+            raw = np.empty(2000, np.float16)
+            assert dev.hip.hipMemcpy(raw.ctypes.data, d.data_ptr() + 4 * at, 4000, 2) == 0
+            assert np.allclose(raw.astype(np.float64), want, rtol=2.0 ** -10, atol=0), at   # lo and lo + 255 * step: one fp16 rounding
+    c.close()
+    e.close()
+
+
 @pytest.mark.parametrize("K,bits,group", [(80, 8, 0), (81, 4, 16), (192, 8, 64), (515, 4, 0)])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_read_with_dropout_is_dropout_of_the_read(dev, dtype, K, bits, group):
@@ -503,7 +524,7 @@ def test_read_with_dropout_is_dropout_of_the_read(dev, dtype, K, bits, group):
     plain = dev.up(np.full(x.size, 3.0), "float64" if dtype == "float64" else "float32")
     c.read(plain, slots=at)
     wide = dev.down(plain, x.shape)
-    for p, seed, offset in ((0.2, 5, 0), (0.5, 6, 1), (0.7, 7, 2 ** 64 - 3), (1.0, 8, 0)):
+    for p, seed, offset in ((0.2, 5, 0), (0.5, 6, 1), (0.7, 7, 2 ** 64 - 3), (1.0, 8, 0), (1e-10, 9, 0)):
         out = dev.up(np.full(x.size, 3.0), dtype)
         c.read(out, slots=at, p=p, seed=seed, offset=offset)
         got = dev.down(out, x.shape)
