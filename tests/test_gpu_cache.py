@@ -387,6 +387,26 @@ def test_refusals(dev):
     e.close()
 
 
+def test_closed_caches_and_engines_are_refused():
+    import gomel_amd
+    e = engine(16)
+    c = e.cache(4)
+    x = np.zeros((1, 16, 2), np.float32)
+    b = gomel_amd.Batch(e, [16])
+    c.close()
+    c.close()
+    for call in (lambda: c.write(x), lambda: c.read(x), c.bad_slots, lambda: b.upload_cache(c, [0]), lambda: e.from_cache(c, [[0]])):
+        with pytest.raises(gomel_amd.GomelError) as err:
+            call()
+        assert err.value.status == 7
+    b.close()
+    e.close()
+    for call in (lambda: e.cache(4), lambda: e.dropout(x, 0.5, 1), lambda: e.dropout_backward(x, 0.5, 1)):
+        with pytest.raises(gomel_amd.GomelError) as err:
+            call()
+        assert err.value.status == 7
+
+
 def test_a_cache_of_more_than_4_gib(dev):
     """Slots whose byte offset does not fit 32 bits."""
     K = 192
@@ -707,6 +727,27 @@ def _torch_child(rep):
         want = want_of(x)
         assert ref.close(out.double().cpu().numpy(), (want, np.abs(want) + 30), "float32", 1)
         assert bool(((z == 0) == (torch.from_numpy(ref.dropped(0.5, 9, 0, z.numel())).to(dev).reshape(z.shape) | (out == 0))).all())
+    # two writes at once on two streams: neighbouring slots of one cache, both by claims, each naming some of its slots twice
+    pair = [torch.cuda.Stream() for _ in range(2)]
+    n = 20000
+    both = e.cache(2 * n, 8, 16)
+    for i in range(4):
+        xs = [torch.randn(n, K, 2, device=dev) for _ in range(2)]
+        at = [2 * torch.randperm(n, device=dev) + k for k in range(2)]
+        for a in at:
+            a[: n // 4] = a[n // 4: n // 2]
+        torch.cuda.synchronize()
+        for k in range(2):
+            with torch.cuda.stream(pair[k]):
+                both.write(xs[k], slots=at[k])
+        torch.cuda.synchronize()
+        for k in range(2):
+            val, out = torch.empty_like(xs[k]), torch.empty_like(xs[k])
+            e.cache(n, 8, 16).write(xs[k], values=val)
+            both.read(out, slots=at[k])
+            assert torch.equal(out[n // 4:], val[n // 4:]), (i, k)
+            assert torch.equal(out[: n // 4], val[n // 4: n // 2]), (i, k)
+    both.close()
     s2 = torch.cuda.Stream()
     x = torch.randn(64, K, 2, device=dev)
     torch.cuda.synchronize()
