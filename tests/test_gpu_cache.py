@@ -708,6 +708,34 @@ def _torch_child(rep):
             continue
         raise AssertionError("not refused: %s" % bad.dtype)
 
+    rep.stage("large calls")                             # outputs, and rows of the cache, that are stored past the caches
+    e192 = engine(192, Device=0)
+    for dtype, bits, group, n in ((torch.bfloat16, 8, 64, 120_000), (torch.bfloat16, 8, 0, 350_000), (torch.float64, 4, 32, 40_000), (torch.float32, 8, 16, 320_000),
+                                  (torch.float16, 4, 0, 100_000)):
+        m = 1000                                         # a thousand frames, again and again: the large call's rows are the small one's
+        base = (torch.randn(m, 192, 2, device=dev) * 3).to(dtype)
+        small, large = e192.cache(m, bits, group), e192.cache(n, bits, group)
+        vs = torch.empty_like(base)
+        small.write(base, values=vs)
+        x = base.repeat(n // m, 1, 1)
+        vl, out, at = torch.empty_like(x), torch.empty_like(x), torch.randperm(n, device=dev)
+        large.write(x, slots=at, values=vl)
+        large.read(out, slots=at)
+        for got in (vl, out):
+            assert torch.equal(got.view(n // m, m, 192, 2), vs.expand(n // m, m, 192, 2)), (dtype, bits, group)
+        large.read(out, slots=at, p=0.25, seed=3)
+        assert torch.equal(out, e192.dropout(vl, 0.25, 3)) or dtype in (torch.float16, torch.bfloat16)
+        y = e192.dropout(x, 0.25, 3)
+        del large
+        wide = torch.empty(n, 390, device=dev, dtype=dtype)
+        assert torch.equal(e192.dropout(x.view(n, 384), 0.25, 3, out=wide[:, 3:387]), y.view(n, 384))
+        per = 2 ** 20                                    # the dense call against calls of a few MB at their offsets
+        for k in (0, x.numel() // per // 2, x.numel() // per - 1):
+            part = x.view(-1)[k * per:(k + 1) * per]
+            assert torch.equal(y.view(-1)[k * per:(k + 1) * per], e192.dropout(part.clone(), 0.25, 3, offset=k * per)), (dtype, k)
+        del x, vl, out, y, wide
+    e192.close()
+
     rep.stage("streams")
     side = torch.cuda.Stream()
     big = torch.randn(4096, 4096, device=dev)
