@@ -43,6 +43,14 @@ def _stream(stream, device):
     return 0 if device is None else _raw_stream(device)
 
 
+def _as_stream(stream, device):
+    """torch's stream object for a `stream` argument (an integer handle, or an object with .cuda_stream)."""
+    if isinstance(stream, _torch.cuda.Stream):
+        return stream
+    handle = int(getattr(stream, "cuda_stream", stream))
+    return _torch.cuda.ExternalStream(handle, device=device) if handle else _torch.cuda.default_stream(device)
+
+
 def _device_of(engine_device, *devices):
     """The device of a call's tensors (None: there are none); they have to be on one device, the engine's."""
     got = None
@@ -227,7 +235,11 @@ def from_cache(engine, cache, slots, x0s=None, seeds=None, stream=None):
     counts = [int(s.numel()) if hasattr(s, "numel") else len(s) for s in slots]
     if not counts:
         return []
-    if any(_is_tensor(s) for s in slots):
+    tensors = [s for s in slots if _is_tensor(s)]
+    if tensors and stream is not None and tensors[0].is_cuda:   # joined in the order of the call's stream: there the slots are ready, and there they are read
+        with _torch.cuda.stream(_as_stream(stream, tensors[0].device)):
+            flat = _torch.cat([s.reshape(-1) for s in slots])
+    elif tensors:
         flat = _torch.cat([s.reshape(-1) for s in slots])
     else:
         flat = np.concatenate([np.asarray(s, dtype=np.int64).reshape(-1) for s in slots])

@@ -1,0 +1,71 @@
+"""GPU tests of how the spectrogram cache and dropout are called: streams, captures, derivatives, calls that fail on the way.  Values are
+held against the definitions (cache_reference.py) or against the same call made one step at a time; what a kernel computes is
+test_gpu_cache.py's subject."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import cache_reference as ref
+from test_gpu_cache import Dev, dev, engine, frames  # noqa: F401  (dev: the fixture)
+
+pytestmark = [pytest.mark.gpu]
+
+
+def _late(torch, stream, n=20):
+    """Work of some milliseconds on `stream`: whatever is queued there behind it happens late."""
+    with torch.cuda.stream(stream):
+        big = torch.randn(4096, 4096, device="cuda")
+        for _ in range(n):
+            big = big @ big
+            big = big / big.norm()
+
+
+# ------------------------------------------------------------------------------------------------ slots made late on a named stream
+def _from_cache_child(rep):
+    import torch
+    rep.stage("torch.cuda init")
+    torch.zeros(1, device="cuda")
+    e = engine(16, Device=0, GriffinLimIterations=2)
+    c = e.cache(64, 8, 0)
+    x = torch.randn(64, 16, 2, device="cuda")
+    c.write(x)
+    side = torch.cuda.Stream()
+    want = e.from_cache(c, [np.arange(8, 20), np.arange(30, 45)], seeds=[1, 2])
+    rep.stage("slots written late on the stream that the call names")
+    for named in (side, side.cuda_stream):
+        at = [torch.zeros(12, dtype=torch.int64, device="cuda"), torch.zeros(15, dtype=torch.int64, device="cuda")]   # slot 0 until then
+        first = [torch.arange(8, 20, device="cuda"), torch.arange(30, 45, device="cuda")]
+        torch.cuda.synchronize()
+        _late(torch, side)
+        with torch.cuda.stream(side):
+            for a, f in zip(at, first):
+                a.copy_(f)
+        got = e.from_cache(c, at, seeds=[1, 2], stream=named)
+        assert all(np.array_equal(g, w) for g, w in zip(got, want))
+    rep.stage("the stream named, the current one busy")
+    torch.cuda.synchronize()
+    _late(torch, torch.cuda.current_stream())
+    got = e.from_cache(c, first, seeds=[1, 2], stream=side)
+    assert all(np.array_equal(g, w) for g, w in zip(got, want))
+    got = e.from_cache(c, first, seeds=[1, 2], stream=0)
+    assert all(np.array_equal(g, w) for g, w in zip(got, want))
+    rep.stage("no stream named: the current one")
+    at = [torch.zeros(12, dtype=torch.int64, device="cuda"), torch.zeros(15, dtype=torch.int64, device="cuda")]
+    torch.cuda.synchronize()
+    _late(torch, side)
+    with torch.cuda.stream(side):
+        for a, f in zip(at, first):
+            a.copy_(f)
+        got = e.from_cache(c, at, seeds=[1, 2])
+    assert all(np.array_equal(g, w) for g, w in zip(got, want))
+    c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_from_cache_joins_its_slots_on_the_stream_of_the_call():
+    import _children
+    assert _children.run_child(_from_cache_child)["ok"]
