@@ -85,6 +85,7 @@ SYMBOLS = {
     "gomel_set_precision_schedule": (ctypes.c_int, [_vp, ctypes.c_int32]),
     "gomel_auto_fp64_iterations": (ctypes.c_int32, [_cfg_p, ctypes.c_int32]),
     "gomel_get_precision": (ctypes.c_int, [_vp, ctypes.c_int32, ctypes.POINTER(ctypes.c_int32)]),
+    "gomel_device": (ctypes.c_int, [_vp]),
     "gomel_cache_frame_bytes": (ctypes.c_size_t, [_cfg_p, ctypes.c_int, ctypes.c_int]),
     "gomel_cache_create": (ctypes.c_int, [_vp, ctypes.c_size_t, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]),
     "gomel_cache_destroy": (ctypes.c_int, [_vp]),

@@ -1166,6 +1166,8 @@ int gomel_destroy(gomel_handle* h) {
     return GOMEL_OK;
 }
 
+int gomel_device(const gomel_handle* h) { return h ? h->device : -1; }
+
 int gomel_device_name(const gomel_handle* h, char* buf, size_t cap) {
     if (!h || !buf || cap == 0) return GOMEL_ERR_NULL;
     hipDeviceProp_t p;

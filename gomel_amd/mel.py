@@ -68,13 +68,14 @@ class Engine:
 
     def __init__(self, cfg, tables=None):
         self._h = ctypes.c_void_p()
-        self.cfg = cfg
+        self.cfg = cfg = GomelConfig.from_buffer_copy(cfg)
         L = _lib.lib()
         if tables is None:
             check(L.gomel_create(ctypes.byref(cfg), ctypes.byref(self._h)), "gomel_create")
         else:
             buf = (ctypes.c_char * len(tables)).from_buffer_copy(tables)
             check(L.gomel_create_from_tables(ctypes.byref(cfg), buf, len(tables), ctypes.byref(self._h)), "gomel_create_from_tables")
+        cfg.device = L.gomel_device(self._h)         # the device itself where the configuration said -1 (the thread's current one)
 
     def close(self):
         """gomel_destroy.  A handle with submitted jobs that have not been waited for refuses (GOMEL_ERR_BUSY): it STAYS valid and this

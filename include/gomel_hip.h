@@ -384,6 +384,8 @@ int gomel_numa_cpus(const char* sysfs_root, const char* pci_bus_id, int32_t* nod
 int gomel_numa_bind_thread(const char* sysfs_root, const char* pci_bus_id, int32_t* node, int32_t* n_bound);
 int gomel_device_count(void);
 int gomel_device_name(const gomel_handle* h, char* buf, size_t cap);
+/* The ordinal of the device a handle works on (its configuration may say -1); -1 for NULL. */
+int gomel_device(const gomel_handle* h);
 /* Blocks until every piece of work queued on `device` by this process has finished (hipDeviceSynchronize with the calling thread's
  * device saved and restored): what a timing harness or a host without its own HIP binding brackets a measurement with.
  * device = -1: the calling thread's current device. */

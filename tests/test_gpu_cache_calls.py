@@ -69,3 +69,39 @@ def _from_cache_child(rep):
 def test_from_cache_joins_its_slots_on_the_stream_of_the_call():
     import _children
     assert _children.run_child(_from_cache_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ an engine whose configuration names no device
+def test_an_engine_knows_its_device():
+    import gomel_amd
+    from gomel_amd import _lib
+    m = gomel_amd.NewMel()
+    assert m.Device == -1
+    cfg = m._config()
+    e = gomel_amd.Engine(cfg)
+    assert cfg.device == -1 and e.cfg.device == 0 == _lib.lib().gomel_device(e._h) and e.cache(4).device == 0
+    e.close()
+
+
+def _vouched_child(rep):
+    import torch
+    torch.zeros(1, device="cuda")
+    import gomel_amd.cache as gc
+    e = engine(16)                                       # Device = -1
+    c = e.cache(8)
+    seen = []
+    write, read = c._write, c._read
+    c._write, c._read = (lambda *a: seen.append(a[1]) or write(*a)), (lambda *a: seen.append(a[1]) or read(*a))
+    x, at = torch.randn(3, 16, 2, device="cuda"), torch.arange(3, device="cuda")
+    v, out = torch.empty_like(x), torch.empty_like(x)
+    c.write(x, slots=at, values=v)
+    c.read(out, slots=at)
+    assert seen == [1 | gc._ON_DEVICE] * 2 and torch.equal(v, out)
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_an_engine_without_a_named_device_vouches_for_its_tensors():
+    import _children
+    assert _children.run_child(_vouched_child)["ok"]
