@@ -35,12 +35,17 @@ def _is_tensor(a):
     return isinstance(a, _Tensor)
 
 
-def _stream(stream, device):
+def _stream(stream, device, engine_device):
     """The hipStream_t a call runs on: `stream` (an integer handle, or an object with .cuda_stream), else torch's current stream of the
-    tensors' device, else the default stream."""
+    tensors' device -- of the engine's, where the call has no tensor: it follows the tensor calls before it --, else the default stream."""
     if stream is not None:
         return int(getattr(stream, "cuda_stream", stream))
-    return 0 if device is None else _raw_stream(device)
+    if device is not None:
+        return _raw_stream(device)
+    cuda = getattr(sys.modules.get("torch"), "cuda", None)      # (torch may not be there, or be on its way in)
+    if engine_device < 0 or cuda is None or not getattr(cuda, "is_initialized", bool)():
+        return 0
+    return cuda.current_stream(engine_device).cuda_stream
 
 
 def _as_stream(stream, device):
@@ -185,7 +190,7 @@ class Cache:
         on = _device_of(self.device, dev, vdev, sdev)
         if on == self.device and dev is not None and (values is None or vdev is not None) and (slots is None or sdev is not None):
             t |= _ON_DEVICE
-        rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, on))
+        rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, on, self.device))
         if rc:
             check(rc, "gomel_cache_write")
         return values
@@ -200,7 +205,7 @@ class Cache:
         on = _device_of(self.device, dev, sdev)
         if on == self.device and dev is not None and (slots is None or sdev is not None):
             t |= _ON_DEVICE
-        rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on))
+        rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on, self.device))
         if rc:
             check(rc, "gomel_cache_read")
         return out
@@ -227,7 +232,8 @@ class Cache:
 def batch_upload_cache(batch, cache, slots, x0s=None, seeds=None, stream=None):
     sp, keep, dev = _slots(slots, sum(batch.n_pairs) // batch.engine.cfg.num_mels)
     xp, xs, seed_p = batch._x0_args(x0s, seeds)
-    check(_lib.lib().gomel_batch_upload_cache(batch._b, cache._c, sp, xp, seed_p, _stream(stream, _device_of(cache.device, dev))), "gomel_batch_upload_cache")
+    check(_lib.lib().gomel_batch_upload_cache(batch._b, cache._c, sp, xp, seed_p, _stream(stream, _device_of(cache.device, dev), cache.device)),
+          "gomel_batch_upload_cache")
     del xs, keep
 
 
@@ -260,7 +266,8 @@ def to_mel_cache(engine, waves, cache, slots, stream=None):
     sp, keep, dev = _slots(slots, total)
     wp = (_lib.c_double_p * len(ws))(*[w.ctypes.data_as(_lib.c_double_p) for w in ws])
     ns = (ctypes.c_size_t * len(ws))(*[w.size for w in ws])
-    check(L.gomel_to_mel_cache(engine._h, len(ws), wp, ns, cache._c, sp, total, _stream(stream, _device_of(cache.device, dev))), "gomel_to_mel_cache")
+    check(L.gomel_to_mel_cache(engine._h, len(ws), wp, ns, cache._c, sp, total, _stream(stream, _device_of(cache.device, dev), cache.device)),
+          "gomel_to_mel_cache")
     del keep
     return counts
 
@@ -288,7 +295,7 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
         t, n = _torch_types.get(x.dtype), x.numel()                       # two dense tensors: nothing to work out
         if t is not None and n and device == x.get_device() == out.get_device():
             rc = fn(engine._h, t | _ON_DEVICE, x.data_ptr(), n, out.data_ptr(), n, 1, n, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
-                    _stream(stream, device))
+                    _stream(stream, device, device))
             if rc:
                 check(rc, where)
             return out
@@ -310,7 +317,7 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
     on = _device_of(device, dev, odev)
     if on == device and dev is not None and odev is not None:
         t |= _ON_DEVICE
-    rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on))
+    rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on, device))
     if rc:
         check(rc, where)
     return out

@@ -1,0 +1,67 @@
+"""CPU tests of how the Python side of the spectrogram cache and dropout makes its calls: the stream it picks, what it refuses, what it
+counts.  The library is replaced by a recorder; nothing here touches a device."""
+import ctypes
+import sys
+import types
+
+import numpy as np
+import pytest
+
+from test_cache import _Engine, _cache
+
+
+def _recording(c=None):
+    """A cache whose library calls land in a list."""
+    c, seen = c or _cache(), []
+    c._write = lambda *a: seen.append(a) or 0
+    c._read = lambda *a: seen.append(a) or 0
+    return c, seen
+
+
+class _Torch(types.ModuleType):
+    """What the choice of a stream asks of torch: cuda.is_initialized, cuda.current_stream(device)."""
+
+    def __init__(self, initialized):
+        super().__init__("torch")
+        self.cuda = types.SimpleNamespace(is_initialized=lambda: initialized, current_stream=lambda d: types.SimpleNamespace(cuda_stream=0x1000 + d))
+
+
+@pytest.mark.skipif("torch" in sys.modules, reason="torch is imported: its place is taken")
+def test_calls_without_a_tensor_run_on_torchs_current_stream(monkeypatch):
+    from gomel_amd import DevicePointer, cache
+    c, seen = _recording()
+    c.device = 3
+    x, d = np.zeros((2, 4, 2)), DevicePointer(4096, 16, "float32")
+
+    def streams():
+        del seen[:]
+        c.write(x)
+        c.read(x, slots=[0, 1])
+        c.write(d, slots=DevicePointer(64, 2, "int64"))
+        c.read(d)
+        c.write(x, stream=7)
+        return [a[-1] for a in seen]
+    assert streams() == [0, 0, 0, 0, 7]                              # no torch in the process
+    monkeypatch.setitem(sys.modules, "torch", _Torch(False))
+    assert streams() == [0, 0, 0, 0, 7]                              # torch, but no GPU context of its own
+    monkeypatch.setitem(sys.modules, "torch", types.ModuleType("torch"))
+    assert streams() == [0, 0, 0, 0, 7]                              # torch half imported
+    monkeypatch.setitem(sys.modules, "torch", _Torch(True))
+    assert streams() == [0x1003] * 4 + [7]
+
+    class Eng(_Engine):
+        class cfg:
+            device = 3
+            num_mels = 4
+    got = []
+    cache._dropout(lambda *a: got.append(a[-1]) or 0, "here", Eng, x, 0.5, 1, 0, None, None)
+    assert got == [0x1003]
+    fake = types.SimpleNamespace(gomel_to_mel_pairs=lambda cfg, n: 4, gomel_to_mel_cache=lambda *a: got.append(a[-1]) or 0,
+                                 gomel_batch_upload_cache=lambda *a: got.append(a[-1]) or 0)
+    monkeypatch.setattr(cache._lib, "lib", lambda: fake)
+    Eng.cfg = ctypes.c_int(0)
+    Eng.cfg.num_mels = 4
+    assert cache.to_mel_cache(Eng, [np.zeros(9)], c, [1]) == [1]
+    batch = types.SimpleNamespace(n_pairs=[4], engine=Eng, _b=None, _x0_args=lambda x0s, seeds: (None, None, None))
+    cache.batch_upload_cache(batch, c, [1])
+    assert got == [0x1003] * 3

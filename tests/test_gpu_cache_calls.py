@@ -105,3 +105,64 @@ def _vouched_child(rep):
 def test_an_engine_without_a_named_device_vouches_for_its_tensors():
     import _children
     assert _children.run_child(_vouched_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ calls without a tensor follow the tensor calls
+def _no_tensor_child(rep):
+    import torch
+    import gomel_amd
+    rep.stage("torch.cuda init")
+    torch.zeros(1, device="cuda")
+    K = 16
+    e = engine(K, Device=0, GriffinLimIterations=2)
+    side = torch.cuda.Stream()
+    x = torch.randn(64, K, 2, device="cuda")
+    c, c2 = e.cache(64, 8, 0), e.cache(64, 8, 0)
+    c2.write(x)
+    want = c2.read(np.empty((64, K, 2), np.float32))
+    waves = e.from_cache(c2, [np.arange(10, 30)], seeds=[5])
+    out = torch.zeros(64, K, 2, device="cuda")
+    for what in ("read", "from_cache", "DevicePointer", "dropout"):
+        rep.stage(what)
+        c.write(torch.zeros_like(x))
+        out.zero_()
+        torch.cuda.synchronize()
+        _late(torch, side)
+        with torch.cuda.stream(side):
+            c.write(x)                                   # late: on the side stream, behind its work
+            if what == "read":
+                assert np.array_equal(c.read(np.empty((64, K, 2), np.float32)), want)
+            elif what == "from_cache":
+                assert np.array_equal(e.from_cache(c, [list(range(10, 30))], seeds=[5])[0], waves[0])
+            elif what == "DevicePointer":
+                c.read(gomel_amd.DevicePointer(out.data_ptr(), out.numel(), "float32"))
+                side.synchronize()
+                assert np.array_equal(out.cpu().numpy(), want)
+            else:
+                c.read(out)
+                y = gomel_amd.DevicePointer(out.data_ptr(), out.numel(), "float32")
+                e.dropout(y, 1.0, 3, out=y)
+                side.synchronize()
+                assert not out.any()
+    rep.stage("to_mel_cache: a tensor read queued before it sees what was there before it")
+    wave = np.random.default_rng(0).normal(size=30000)
+    n = e.to_mel_cache([wave], c, np.arange(len(e.to_mel_batch([wave])[0]) // K))[0]
+    c.write(x)
+    torch.cuda.synchronize()
+    _late(torch, side)
+    with torch.cuda.stream(side):
+        c.read(out)
+        e.to_mel_cache([wave], c, list(range(n)))
+        side.synchronize()
+    assert np.array_equal(out.cpu().numpy(), want)
+    for k in (c, c2):
+        k.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_calls_without_a_tensor_follow_the_current_stream():
+    import _children
+    assert _children.run_child(_no_tensor_child)["ok"]
