@@ -14,7 +14,7 @@ from .mel import Batch, DevicePointer
 
 _ON_DEVICE = 0x100           # GOMEL_DEVICE_MEMORY: nothing of the call is in host memory
 _TYPES = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}
-_torch = None                # the module, once a tensor has been seen
+_torch = _forward_ad = None  # the modules torch and torch.autograd.forward_ad, once a tensor has been seen
 _Tensor = None               # its Tensor type
 _torch_types, _int64 = {}, None
 _raw_stream = None           # device index -> hipStream_t of torch's current stream
@@ -22,14 +22,14 @@ _raw_stream = None           # device index -> hipStream_t of torch's current st
 
 def _is_tensor(a):
     """Whether `a` is a torch tensor (torch is never imported for the question)."""
-    global _torch, _Tensor, _int64, _raw_stream
+    global _torch, _Tensor, _int64, _raw_stream, _forward_ad
     if _Tensor is not None:
         return isinstance(a, _Tensor)
     if "torch" not in sys.modules or not hasattr(a, "data_ptr") or isinstance(a, DevicePointer):
         return False
     import torch
     _torch_types.update({torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3})
-    _int64 = torch.int64
+    _int64, _forward_ad = torch.int64, torch.autograd.forward_ad
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
     _torch, _Tensor = torch, torch.Tensor
     return isinstance(a, _Tensor)
@@ -335,26 +335,35 @@ def _dropout_function():
         class Dropout(torch.autograd.Function):
             @staticmethod
             def forward(ctx, x, engine, p, seed, offset, back):
-                ctx.args = (engine, p, seed, offset, not back)
+                ctx.args, ctx.back = (engine, p, seed, offset), back
                 fn = _lib.lib().gomel_dropout_backward if back else _lib.lib().gomel_dropout
                 return _dropout(fn, "gomel_dropout_backward" if back else "gomel_dropout", engine, x, p, seed, offset, None, None)
 
             @staticmethod
             def backward(ctx, dy):
-                return (Dropout.apply(dy if dy.is_contiguous() else dy.contiguous(), *ctx.args),) + (None,) * 5
+                return (Dropout.apply(dy.contiguous(), *ctx.args, not ctx.back),) + (None,) * 5
+
+            @staticmethod
+            def jvp(ctx, dx, *rest):                     # linear in x: the tangent goes the same way
+                return Dropout.apply(dx.contiguous(), *ctx.args, ctx.back)
 
         _function = Dropout
     return _function
 
 
 def _wants_grad(x):
-    return getattr(x, "requires_grad", False) and sys.modules["torch"].is_grad_enabled()
+    """Whether autograd has to see what is computed from x: in reverse mode, or in forward mode (x carries a tangent)."""
+    if not _is_tensor(x):
+        return False
+    if x.requires_grad and _torch.is_grad_enabled():
+        return True
+    return getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(x).tangent is not None
 
 
 def dropout(engine, x, p, seed, offset=0, out=None, stream=None):
     if _wants_grad(x):
         if out is not None or stream is not None:
-            raise ValueError("out, stream: not with a tensor that requires a gradient")
+            raise ValueError("out, stream: not with a tensor that requires a gradient or carries a tangent")
         return _dropout_function().apply(x, engine, p, seed, offset, False)
     return _dropout(_lib.lib().gomel_dropout, "gomel_dropout", engine, x, p, seed, offset, out, stream)
 
@@ -362,6 +371,6 @@ def dropout(engine, x, p, seed, offset=0, out=None, stream=None):
 def dropout_backward(engine, dy, p, seed, offset=0, out=None, stream=None):
     if _wants_grad(dy):
         if out is not None or stream is not None:
-            raise ValueError("out, stream: not with a tensor that requires a gradient")
+            raise ValueError("out, stream: not with a tensor that requires a gradient or carries a tangent")
         return _dropout_function().apply(dy, engine, p, seed, offset, True)
     return _dropout(_lib.lib().gomel_dropout_backward, "gomel_dropout_backward", engine, dy, p, seed, offset, out, stream)

@@ -65,3 +65,48 @@ def test_calls_without_a_tensor_run_on_torchs_current_stream(monkeypatch):
     batch = types.SimpleNamespace(n_pairs=[4], engine=Eng, _b=None, _x0_args=lambda x0s, seeds: (None, None, None))
     cache.batch_upload_cache(batch, c, [1])
     assert got == [0x1003] * 3
+
+
+# ------------------------------------------------------------------------------------------------ derivatives (torch, in a child process)
+def _derivatives_child(rep):
+    """What autograd makes of Engine.dropout, the kernel replaced by its definition in numpy (it sees values only, as the kernel does)."""
+    import torch
+    import torch.autograd.forward_ad as fwd
+    from gomel_amd import cache
+    import cache_reference as ref
+
+    def kernel(fn, where, engine, x, p, seed, offset, out, stream):
+        v = x.detach().numpy()
+        y = np.where(ref.dropped(p, seed, offset, v.size).reshape(v.shape), 0.0, v / (1 - p))
+        return torch.from_numpy(y.astype(v.dtype))
+    cache._dropout = kernel
+    x, dx, dy = (torch.randn(5, 8, dtype=torch.float64) for _ in range(3))
+    for call in (cache.dropout, cache.dropout_backward):
+        f = lambda t: call(_Engine, t, 0.4, 11, 3)      # noqa: E731
+        want = f(dx)
+        with fwd.dual_level():
+            y = fwd.unpack_dual(f(fwd.make_dual(x, dx)))
+            assert torch.equal(y.primal, f(x)) and y.tangent is not None and torch.equal(y.tangent, want)
+            y = fwd.unpack_dual(f(fwd.make_dual(x, dx[:1].expand(5, 8))))          # a tangent that is not dense
+            assert torch.equal(y.tangent, f(dx[:1].expand(5, 8).contiguous()))
+            assert fwd.unpack_dual(f(x)).tangent is None
+            with torch.no_grad():
+                assert torch.equal(fwd.unpack_dual(f(fwd.make_dual(x, dx))).tangent, want)
+            for kw in ({"out": torch.empty_like(x)}, {"stream": 5}):
+                with pytest.raises(ValueError):
+                    call(_Engine, fwd.make_dual(x, dx), 0.4, 11, 3, **kw)
+        xr = x.clone().requires_grad_(True)
+        with fwd.dual_level():                           # both modes at once: the gradient of a directional derivative
+            (g,) = torch.autograd.grad((f(fwd.make_dual(xr, dx)) ** 2).sum(), xr)
+            t = fwd.unpack_dual(g)
+            assert torch.equal(t.primal, 2 * f(f(x))) and torch.equal(t.tangent, 2 * f(f(dx)))
+        (g,) = torch.autograd.grad(f(xr), xr, dy)
+        assert torch.equal(g, f(dy))
+        assert torch.autograd.gradcheck(f, (xr,), check_forward_ad=True, check_batched_grad=False)
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+def test_dropouts_derivatives_in_both_modes():
+    import _children
+    assert _children.run_child(_derivatives_child)["ok"]

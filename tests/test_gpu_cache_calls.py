@@ -166,3 +166,28 @@ def _no_tensor_child(rep):
 def test_calls_without_a_tensor_follow_the_current_stream():
     import _children
     assert _children.run_child(_no_tensor_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ derivatives
+def _forward_mode_child(rep):
+    import torch
+    import torch.autograd.forward_ad as fwd
+    torch.zeros(1, device="cuda")
+    e = engine(16, Device=0)
+    x, dx = (torch.randn(33, 7, device="cuda", dtype=torch.float64) for _ in range(2))
+    with fwd.dual_level():
+        y = fwd.unpack_dual(e.dropout(fwd.make_dual(x, dx), 0.3, 5, 2))
+        assert torch.equal(y.primal, e.dropout(x, 0.3, 5, 2)) and torch.equal(y.tangent, e.dropout(dx, 0.3, 5, 2))
+        y = fwd.unpack_dual(e.dropout_backward(fwd.make_dual(x, dx), 0.3, 5, 2))
+        assert torch.equal(y.tangent, e.dropout(dx, 0.3, 5, 2))
+    small = torch.randn(11, device="cuda", dtype=torch.float64, requires_grad=True)
+    assert torch.autograd.gradcheck(lambda t: e.dropout(t, 0.4, 2), (small,), check_forward_ad=True)
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_dropout_in_forward_mode():
+    import _children
+    assert _children.run_child(_forward_mode_child)["ok"]
