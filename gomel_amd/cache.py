@@ -136,6 +136,12 @@ def _rows(a, cols, what, write=False):
     return ptr, t, step, rows, device
 
 
+def _output(a, what):
+    """Refuses an output that autograd keeps track of: it does not see what a call writes."""
+    if _wants_grad(a):
+        raise ValueError("%s: a tensor that requires a gradient or carries a tangent cannot be written to" % what)
+
+
 def _slots(slots, n, what="slots"):
     """(address, the array that has to stay alive, device) of one int64 per frame."""
     if _is_tensor(slots):
@@ -176,12 +182,16 @@ class Cache:
 
     def write(self, frames, slots=None, first=0, values=None, stream=None):
         """Quantises `frames` ([n, NumMels, 2] or [n * NumMels, 2]) into their slots.  `values` (same shape and type; may be `frames` itself)
-        receives what the cache now stands for, and is returned."""
+        receives what the cache now stands for, and is returned.  No gradient goes through the quantiser: frames that require one are refused
+        where `values` is given (write frames.detach(); straight through, frames + (values - frames).detach())."""
         cols = 2 * self.num_mels
         ptr, t, stride, n, dev = _rows(frames, cols, "frames")
         sp, keep, sdev = (0, None, None) if slots is None else _slots(slots, n)
         vp, vs, vdev = 0, cols, None
         if values is not None:
+            if _wants_grad(frames):
+                raise ValueError("values: not with frames that require a gradient or carry a tangent")
+            _output(values, "values")
             vp, vt, vs, vn, vdev = _rows(values, cols, "values", write=True)
             if vt != t or vn != n:
                 raise ValueError("values: the frames' type and number of frames are needed")
@@ -198,6 +208,7 @@ class Cache:
     def read(self, out, slots=None, first=0, p=0.0, seed=0, offset=0, stream=None):
         """Dequantises frames into `out` ([n, NumMels, 2] or [n * NumMels, 2]) and returns it.  p > 0: with dropout, as Engine.dropout of
         the dense result."""
+        _output(out, "out")
         ptr, t, stride, n, dev = _rows(out, 2 * self.num_mels, "out", write=True)
         sp, keep, sdev = (0, None, None) if slots is None else _slots(slots, n)
         if first < 0:
@@ -291,6 +302,8 @@ def _flat(a, what, write=False):
 
 def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
     device = engine.cfg.device
+    if out is not None:
+        _output(out, "out")
     if out is not None and _is_tensor(x) and _is_tensor(out) and x.is_contiguous() and out.is_contiguous() and x.shape == out.shape and x.dtype == out.dtype:
         t, n = _torch_types.get(x.dtype), x.numel()                       # two dense tensors: nothing to work out
         if t is not None and n and device == x.get_device() == out.get_device():

@@ -297,8 +297,7 @@ int gomel_get_precision(const gomel_handle* h, int32_t iterations, int32_t* fp64
  * buffer and returns when it is done (not while `stream` is being captured: GOMEL_ERR_BAD_CONFIG).  Calls that touch the same
  * slots on different streams are the caller's to order.  `n` = 0 is a call without work.
  *   gomel_cache_write: quantises n frames.  values != NULL also receives what the cache now stands for, rounded to `type` (what a
- * generating model is to be conditioned on; the forward of training through the quantiser, whose straight-through gradient is the
- * identity); values may be frames itself (same stride) but must not overlap it otherwise.
+ * generating model is to be conditioned on; a straight-through gradient of it is the identity); values may be frames itself (same stride) but must not overlap it otherwise.
  *   gomel_cache_read: dequantises n frames (fp32 arithmetic; fp64 for GOMEL_F64), rounded once to `type`.  p > 0 applies dropout
  * (below) to the values read, element index = position in the dense [n][2 * NumMels] output.
  * The cache keeps nothing of the handle (its NumMels and device are copied): either may be destroyed first. */

@@ -110,3 +110,49 @@ def _derivatives_child(rep):
 def test_dropouts_derivatives_in_both_modes():
     import _children
     assert _children.run_child(_derivatives_child)["ok"]
+
+
+def _tracked_tensors_child(rep):
+    """Calls that autograd would have to see, and does not, are refused before anything is written; the rest go through."""
+    import torch
+    import torch.autograd.forward_ad as fwd
+    from gomel_amd import cache
+    t = torch.randn(3, 4, 2)
+    t.requires_grad_(True)
+    plain = torch.randn(3, 4, 2)
+    rows = cache._rows
+
+    def taken(a, cols, what, write=False):               # CPU tensors as the GPU's
+        return (a.data_ptr(), 1, 8, 3, 0) if cache._is_tensor(a) else rows(a, cols, what, write)
+    cache._rows = taken
+    c, seen = _recording()
+    np_out = np.zeros((3, 4, 2), np.float32)
+    for frames, values in ((t, plain), (t, t), (plain, t), (t * 2, plain), (plain, t * 2), (t * 2, np_out)):
+        with pytest.raises(ValueError, match="gradient"):
+            c.write(frames, values=values, stream=1)
+    for out in (t, t * 2):
+        with pytest.raises(ValueError, match="gradient"):
+            c.read(out, stream=1)
+        with pytest.raises(ValueError, match="gradient"):
+            cache.dropout(_Engine, plain, 0.5, 1, out=out, stream=1)
+        with pytest.raises(ValueError, match="gradient"):
+            cache.dropout_backward(_Engine, plain, 0.5, 1, out=out, stream=1)
+    with fwd.dual_level():
+        d = fwd.make_dual(plain, torch.ones_like(plain))
+        for call in (lambda: c.write(d, values=torch.empty(3, 4, 2), stream=1), lambda: c.write(t.detach(), values=d, stream=1), lambda: c.read(d, stream=1)):
+            with pytest.raises(ValueError, match="tangent"):
+                call()
+    assert seen == []
+    c.write(t, stream=1)                                 # nothing comes back: nothing to differentiate
+    c.write(t.detach(), values=plain, stream=1)
+    with torch.no_grad():
+        c.write(t, values=plain, stream=1)
+        c.read(t, stream=1)
+    assert len(seen) == 4
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+def test_tensors_that_autograd_follows_are_not_written_behind_its_back():
+    import _children
+    assert _children.run_child(_tracked_tensors_child)["ok"]
