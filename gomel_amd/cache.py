@@ -15,21 +15,45 @@ from .mel import Batch, DevicePointer
 _ON_DEVICE = 0x100           # GOMEL_DEVICE_MEMORY: nothing of the call is in host memory
 _TYPES = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}
 _torch = _forward_ad = None  # the modules torch and torch.autograd.forward_ad, once a tensor has been seen
+_increment_version = None    # torch.autograd.graph.increment_version of an iterable of tensors
 _Tensor = None               # its Tensor type
 _torch_types, _int64 = {}, None
 _raw_stream = None           # device index -> hipStream_t of torch's current stream
 
 
+class _AnyLevel:
+    """torch.autograd.forward_ad, where it does not say whether a level of dual tensors is open: every tensor is asked."""
+    _current_level = 0
+
+    @staticmethod
+    def unpack_dual(t):
+        return _torch.autograd.forward_ad.unpack_dual(t)
+
+
+def _version_counter(torch):
+    """torch.autograd.graph.increment_version without its wrapper (0.2 us), where that does the same."""
+    try:
+        probe = torch.empty(0)
+        torch._C._increment_version((probe,))
+        if probe._version == 1:
+            return torch._C._increment_version
+    except (AttributeError, TypeError):
+        pass
+    return torch.autograd.graph.increment_version
+
+
 def _is_tensor(a):
     """Whether `a` is a torch tensor (torch is never imported for the question)."""
-    global _torch, _Tensor, _int64, _raw_stream, _forward_ad
+    global _torch, _Tensor, _int64, _raw_stream, _forward_ad, _increment_version
     if _Tensor is not None:
         return isinstance(a, _Tensor)
     if "torch" not in sys.modules or not hasattr(a, "data_ptr") or isinstance(a, DevicePointer):
         return False
     import torch
     _torch_types.update({torch.float64: 0, torch.float32: 1, torch.float16: 2, torch.bfloat16: 3})
-    _int64, _forward_ad = torch.int64, torch.autograd.forward_ad
+    _int64 = torch.int64
+    _forward_ad = torch.autograd.forward_ad if hasattr(torch.autograd.forward_ad, "_current_level") else _AnyLevel
+    _increment_version = _version_counter(torch)
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
     _torch, _Tensor = torch, torch.Tensor
     return isinstance(a, _Tensor)
@@ -71,9 +95,9 @@ def _rows(a, cols, what, write=False):
     """(address, type code, row stride in elements, rows, device) of an array of rows of `cols` elements.  Rows may be apart; the
     elements of a row are consecutive.  device: a torch tensor's, None otherwise."""
     device = None
-    if _is_tensor(a):
+    if _is_tensor(a) if _Tensor is None else isinstance(a, _Tensor):
         device, t = a.get_device(), _torch_types.get(a.dtype)
-        if device < 0 or not a.is_cuda:
+        if device < 0:
             raise ValueError("%s: a torch tensor must be on the GPU (numpy arrays are taken from host memory)" % what)
         if t is not None and a.is_contiguous():
             rows, rest = divmod(a.numel(), cols)
@@ -142,9 +166,15 @@ def _output(a, what):
         raise ValueError("%s: a tensor that requires a gradient or carries a tangent cannot be written to" % what)
 
 
+def _written(a):
+    """Tells autograd that a call has written to `a`: where it holds the tensor's old values for a backward pass, that pass now raises."""
+    if _Tensor is not None and isinstance(a, _Tensor):
+        _increment_version((a,))
+
+
 def _slots(slots, n, what="slots"):
     """(address, the array that has to stay alive, device) of one int64 per frame."""
-    if _is_tensor(slots):
+    if _is_tensor(slots) if _Tensor is None else isinstance(slots, _Tensor):
         device = slots.get_device()
         if device < 0 or slots.dtype != _int64 or not slots.is_contiguous() or slots.numel() != n:
             raise ValueError("%s: a contiguous int64 CUDA tensor with %d elements is needed" % (what, n))
@@ -197,10 +227,13 @@ class Cache:
                 raise ValueError("values: the frames' type and number of frames are needed")
         if first < 0:
             raise ValueError("first is negative")
-        on = _device_of(self.device, dev, vdev, sdev)
-        if on == self.device and dev is not None and (values is None or vdev is not None) and (slots is None or sdev is not None):
+        on = self.device
+        if dev == on and (values is None or vdev == on) and (slots is None or sdev == on):
             t |= _ON_DEVICE
+        else:
+            on = _device_of(on, dev, vdev, sdev)
         rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, on, self.device))
+        _written(values)
         if rc:
             check(rc, "gomel_cache_write")
         return values
@@ -213,10 +246,13 @@ class Cache:
         sp, keep, sdev = (0, None, None) if slots is None else _slots(slots, n)
         if first < 0:
             raise ValueError("first is negative")
-        on = _device_of(self.device, dev, sdev)
-        if on == self.device and dev is not None and (slots is None or sdev is not None):
+        on = self.device
+        if dev == on and (slots is None or sdev == on):
             t |= _ON_DEVICE
+        else:
+            on = _device_of(on, dev, sdev)
         rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on, self.device))
+        _written(out)
         if rc:
             check(rc, "gomel_cache_read")
         return out
@@ -302,13 +338,14 @@ def _flat(a, what, write=False):
 
 def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
     device = engine.cfg.device
-    if out is not None:
+    if out is not None and (_Tensor is None or not isinstance(out, _Tensor) or out.requires_grad or _forward_ad._current_level >= 0):
         _output(out, "out")
-    if out is not None and _is_tensor(x) and _is_tensor(out) and x.is_contiguous() and out.is_contiguous() and x.shape == out.shape and x.dtype == out.dtype:
+    if out is not None and _Tensor is not None and isinstance(x, _Tensor) and isinstance(out, _Tensor) and x.is_contiguous() and out.is_contiguous() and x.shape == out.shape and x.dtype == out.dtype:
         t, n = _torch_types.get(x.dtype), x.numel()                       # two dense tensors: nothing to work out
         if t is not None and n and device == x.get_device() == out.get_device():
             rc = fn(engine._h, t | _ON_DEVICE, x.data_ptr(), n, out.data_ptr(), n, 1, n, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
-                    _stream(stream, device, device))
+                    _raw_stream(device) if stream is None else _stream(stream, device, device))
+            _increment_version((out,))
             if rc:
                 check(rc, where)
             return out
@@ -331,6 +368,7 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
     if on == device and dev is not None and odev is not None:
         t |= _ON_DEVICE
     rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on, device))
+    _written(out)
     if rc:
         check(rc, where)
     return out
@@ -366,11 +404,11 @@ def _dropout_function():
 
 def _wants_grad(x):
     """Whether autograd has to see what is computed from x: in reverse mode, or in forward mode (x carries a tangent)."""
-    if not _is_tensor(x):
+    if not (_is_tensor(x) if _Tensor is None else isinstance(x, _Tensor)):
         return False
     if x.requires_grad and _torch.is_grad_enabled():
         return True
-    return getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(x).tangent is not None
+    return _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(x).tangent is not None
 
 
 def dropout(engine, x, p, seed, offset=0, out=None, stream=None):

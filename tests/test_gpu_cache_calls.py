@@ -186,6 +186,44 @@ def _forward_mode_child(rep):
     rep.result({"ok": True})
 
 
+def _versions_child(rep):
+    """A buffer that autograd holds for a backward pass and a call then writes to: that pass raises, as after torch's own in-place writes."""
+    import torch
+    torch.zeros(1, device="cuda")
+    e = engine(16, Device=0)
+    c = e.cache(8)
+    w = torch.randn(16, 2, device="cuda", requires_grad=True)
+    c.write(torch.randn(3, 16, 2, device="cuda"))
+    for write in (lambda b: c.read(b), lambda b: c.read(b, p=0.5, seed=1), lambda b: c.write(torch.randn_like(b), values=b), lambda b: c.write(b, values=b),
+                  lambda b: e.dropout(torch.randn_like(b), 0.5, 1, out=b), lambda b: e.dropout_backward(b, 0.5, 1, out=b),
+                  lambda b: e.dropout(torch.randn_like(b), 0.5, 1, out=b, stream=torch.cuda.current_stream()),
+                  lambda b: c.read(b.view(3, 32).view(3, 16, 2))):
+        buf = torch.randn(3, 16, 2, device="cuda")
+        loss = (w * buf).sum()                               # the product holds buf
+        write(buf)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            loss.backward()
+    buf = torch.randn(3, 16, 2, device="cuda")
+    loss = (w * buf).sum()
+    c.write(buf)                                             # only read: nothing to tell
+    e.dropout(buf, 0.5, 1)
+    loss.backward()
+    with torch.inference_mode():                             # tensors without a version
+        buf = torch.randn(3, 16, 2, device="cuda")
+        c.read(buf)
+        c.write(buf, values=buf)
+        e.dropout(buf, 0.5, 1, out=buf)
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_autograd_sees_what_a_call_has_written():
+    import _children
+    assert _children.run_child(_versions_child)["ok"]
+
+
 @pytest.mark.torch_child
 @pytest.mark.guard(700)
 def test_dropout_in_forward_mode():
