@@ -80,6 +80,13 @@ def _as_stream(stream, device):
     return _torch.cuda.ExternalStream(handle, device=device) if handle else _torch.cuda.default_stream(device)
 
 
+def _used_on(stream, *arrays):
+    """Tells torch's allocator that a call on a named stream still uses these tensors: their memory is not handed on before it is through."""
+    for a in arrays:
+        if _Tensor is not None and isinstance(a, _Tensor):
+            a.record_stream(_as_stream(stream, a.device))
+
+
 def _device_of(engine_device, *devices):
     """The device of a call's tensors (None: there are none); they have to be on one device, the engine's."""
     got = None
@@ -234,6 +241,8 @@ class Cache:
             on = _device_of(on, dev, vdev, sdev)
         rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, on, self.device))
         _written(values)
+        if stream is not None:
+            _used_on(stream, frames, values, slots)
         if rc:
             check(rc, "gomel_cache_write")
         return values
@@ -253,6 +262,8 @@ class Cache:
             on = _device_of(on, dev, sdev)
         rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on, self.device))
         _written(out)
+        if stream is not None:
+            _used_on(stream, out, slots)
         if rc:
             check(rc, "gomel_cache_read")
         return out
@@ -346,6 +357,8 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
             rc = fn(engine._h, t | _ON_DEVICE, x.data_ptr(), n, out.data_ptr(), n, 1, n, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
                     _raw_stream(device) if stream is None else _stream(stream, device, device))
             _increment_version((out,))
+            if stream is not None:
+                _used_on(stream, x, out)
             if rc:
                 check(rc, where)
             return out
@@ -369,6 +382,8 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
         t |= _ON_DEVICE
     rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on, device))
     _written(out)
+    if stream is not None:
+        _used_on(stream, x, out)
     if rc:
         check(rc, where)
     return out

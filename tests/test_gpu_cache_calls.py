@@ -229,3 +229,51 @@ def test_autograd_sees_what_a_call_has_written():
 def test_dropout_in_forward_mode():
     import _children
     assert _children.run_child(_forward_mode_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ tensors dropped while a named stream uses them
+def _dropped_tensors_child(rep):
+    import torch
+    torch.zeros(1, device="cuda")
+    K, n = 80, 3000
+    e = engine(K, Device=0)
+    c = e.cache(n)
+    base = torch.randn(n, K, 2, device="cuda", dtype=torch.float64)
+    at = torch.randperm(n, device="cuda", dtype=torch.int64)
+    want, y_want = torch.empty(n, K, 2, device="cuda"), torch.empty(n, K, 2, device="cuda")
+    c.write(base.float(), values=want)
+    e.dropout(base.float(), 0.5, 1, out=y_want)
+    side = torch.cuda.Stream()
+
+    def others(*like):                                   # memory of these sizes, freed just now, goes to somebody else at once
+        return [torch.full_like(t, 7) for t in like for _ in range(3)]
+    for named in (side, side.cuda_stream):
+        c.write(torch.zeros_like(want))
+        out, y, val = (torch.empty_like(want) for _ in range(3))
+        like, like_at = torch.empty_like(want), torch.empty_like(at)
+        torch.cuda.synchronize()
+        _late(torch, side)
+        x, x2, at1, at2 = base.float(), base.float(), at.clone(), at.clone()
+        side.wait_stream(torch.cuda.current_stream())
+        c.write(x, slots=at1, values=val, stream=named)
+        c.read(out, slots=at2, stream=named)
+        e.dropout(x2, 0.5, 1, out=y, stream=named)
+        del x, x2, at1, at2
+        held = others(like, like_at)
+        c.read(torch.empty_like(out), stream=named)      # an output that nobody keeps: it must not be written over somebody else's memory
+        held += others(like)
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(val, want) and torch.equal(y, y_want)
+        assert all(bool((h == 7).all()) for h in held)
+        del held
+    c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_tensors_dropped_while_a_named_stream_uses_them():
+    import _children
+    assert _children.run_child(_dropped_tensors_child)["ok"]
