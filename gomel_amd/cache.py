@@ -9,7 +9,7 @@ import sys
 import numpy as np
 
 from . import _lib
-from ._lib import check
+from ._lib import GomelError, check
 from .mel import Batch, DevicePointer
 
 _ON_DEVICE = 0x100           # GOMEL_DEVICE_MEMORY: nothing of the call is in host memory
@@ -59,6 +59,21 @@ def _is_tensor(a):
     return isinstance(a, _Tensor)
 
 
+def _torch_cuda():
+    """torch.cuda where this process uses it, else None (torch may not be there, or be on its way in)."""
+    cuda = getattr(sys.modules.get("torch"), "cuda", None)
+    return cuda if cuda is not None and getattr(cuda, "is_initialized", bool)() else None
+
+
+def _capturing(stream, device):
+    """Whether torch's current stream, or the stream a call names, is being captured into a graph."""
+    cuda = _torch_cuda()
+    if cuda is None:
+        return False
+    with cuda.stream(cuda.current_stream(device) if stream is None else _as_stream(stream, device)):
+        return cuda.is_current_stream_capturing()
+
+
 def _stream(stream, device, engine_device):
     """The hipStream_t a call runs on: `stream` (an integer handle, or an object with .cuda_stream), else torch's current stream of the
     tensors' device -- of the engine's, where the call has no tensor: it follows the tensor calls before it --, else the default stream."""
@@ -66,18 +81,17 @@ def _stream(stream, device, engine_device):
         return int(getattr(stream, "cuda_stream", stream))
     if device is not None:
         return _raw_stream(device)
-    cuda = getattr(sys.modules.get("torch"), "cuda", None)      # (torch may not be there, or be on its way in)
-    if engine_device < 0 or cuda is None or not getattr(cuda, "is_initialized", bool)():
-        return 0
-    return cuda.current_stream(engine_device).cuda_stream
+    cuda = _torch_cuda()
+    return 0 if cuda is None or engine_device < 0 else cuda.current_stream(engine_device).cuda_stream
 
 
 def _as_stream(stream, device):
     """torch's stream object for a `stream` argument (an integer handle, or an object with .cuda_stream)."""
-    if isinstance(stream, _torch.cuda.Stream):
+    cuda = sys.modules["torch"].cuda
+    if isinstance(stream, cuda.Stream):
         return stream
     handle = int(getattr(stream, "cuda_stream", stream))
-    return _torch.cuda.ExternalStream(handle, device=device) if handle else _torch.cuda.default_stream(device)
+    return cuda.ExternalStream(handle, device=device) if handle else cuda.default_stream(device)
 
 
 def _used_on(stream, *arrays):
@@ -299,6 +313,8 @@ def from_cache(engine, cache, slots, x0s=None, seeds=None, stream=None):
     counts = [int(s.numel()) if hasattr(s, "numel") else len(s) for s in slots]
     if not counts:
         return []
+    if _capturing(stream, cache.device):         # as gomel_batch_upload_cache, before a batch is allocated
+        raise GomelError(1, "from_cache")
     tensors = [s for s in slots if _is_tensor(s)]
     if tensors and stream is not None and tensors[0].is_cuda:   # joined in the order of the call's stream: there the slots are ready, and there they are read
         with _torch.cuda.stream(_as_stream(stream, tensors[0].device)):

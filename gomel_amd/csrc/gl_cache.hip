@@ -721,13 +721,6 @@ struct OnDevice {   // the calling thread's device switched to `dev` and back
 int hip_failed(hipError_t e) { g_last_hip = (int)e; (void)hipGetLastError(); return GOMEL_ERR_HIP; }
 #define CHK(expr) do { const hipError_t e_ = (expr); if (e_ != hipSuccess) return hip_failed(e_); } while (0)
 
-bool capturing(hipStream_t s) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (!s) return false;
-    if (hipStreamIsCapturing(s, &st) != hipSuccess) { (void)hipGetLastError(); return false; }
-    return st != hipStreamCaptureStatusNone;
-}
-
 hipError_t dropout_device(int type, const void* x, size_t xs, void* y, size_t ys, size_t rows, size_t cols, const DropRule& d, uint64_t seed, uint64_t offset, hipStream_t s) {
     const size_t total = rows * cols, bytes = total * (size_t)type_bytes(type), uv = 16 / (size_t)type_bytes(type);
     DropArgs a{x, y, (int64_t)xs, (int64_t)ys, (int64_t)cols, (int64_t)total, Walk{}, d, seed, offset, (int32_t)(offset + (uint64_t)total < offset)};
@@ -792,7 +785,7 @@ int cache_call(gomel_cache* c, int type, const void* in, size_t is, void* out, s
     const int ki = in ? memory_kind(in, c->device) : 1, ko = out ? memory_kind(out, c->device) : 1, ks = slots ? memory_kind(slots, c->device) : 1;
     if (ki < 0 || ko < 0 || ks < 0) return GOMEL_ERR_BAD_CONFIG;
     if (ki && ko && ks) { CHK(run(type, in, is, out, os, n, slots, first)); return GOMEL_OK; }
-    if (capturing(s)) return GOMEL_ERR_BAD_CONFIG;
+    if (stream_capturing(s)) return GOMEL_ERR_BAD_CONFIG;
     if (!ks) { const int rc = check_slots(slots, n, c->n_slots, true); if (rc) return rc; }
     std::lock_guard<std::mutex> lk(c->mu);
     const size_t row = cols * esz, piece = std::min(n, std::max<size_t>(1, kStageBytes / row));
@@ -868,7 +861,7 @@ int dropout_call(gomel_handle* h, int type, const void* x, size_t xs, void* y, s
     const int kx = vouched ? 1 : memory_kind(x, device), ky = vouched ? 1 : memory_kind(y, device);
     if (kx < 0 || ky < 0) return GOMEL_ERR_BAD_CONFIG;
     if (kx && ky) { CHK(dropout_device(type, x, xs, y, ys, rows, cols, d, seed, offset, s)); return GOMEL_OK; }
-    if (capturing(s)) return GOMEL_ERR_BAD_CONFIG;
+    if (stream_capturing(s)) return GOMEL_ERR_BAD_CONFIG;
     // pieces of whole rows, or of one row where a row alone is larger than the staging buffer
     const size_t row = cols * esz, pr = std::max<size_t>(1, kStageBytes / row), pc = row > kStageBytes ? kStageBytes / esz : cols;
     const size_t bytes = std::min(rows, pr) * std::min(cols, pc) * esz;
@@ -899,6 +892,13 @@ int memory_kind(const void* p, int device) {
     if (hipPointerGetAttributes(&at, p) != hipSuccess) { (void)hipGetLastError(); return 0; }
     if (at.type == hipMemoryTypeDevice) return at.device == device ? 1 : -1;
     return 0;   // pageable, pinned and managed memory go through the staging buffer
+}
+
+bool stream_capturing(hipStream_t s) {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (!s) return false;
+    if (hipStreamIsCapturing(s, &st) != hipSuccess) { (void)hipGetLastError(); return false; }
+    return st != hipStreamCaptureStatusNone;
 }
 
 hipError_t cache_write_device(gomel_cache* c, int type, const void* x, size_t xs, size_t n, const int64_t* slots, size_t first, void* y, size_t ys, hipStream_t s) {

@@ -28,6 +28,8 @@ GL_HIDDEN hipError_t cache_read_device(gomel_cache* c, int type, void* y, size_t
                                        uint64_t seed, uint64_t offset, bool strict, unsigned long long* bad, hipStream_t s);
 // what kind of memory p is: 1 = memory of `device`, 0 = host memory, -1 = memory of another device
 GL_HIDDEN int memory_kind(const void* p, int device);
+// whether s is being captured into a graph
+GL_HIDDEN bool stream_capturing(hipStream_t s);
 
 // defined in gomel_hip.hip
 GL_HIDDEN int handle_device(const gomel_handle* h);

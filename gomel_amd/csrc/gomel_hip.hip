@@ -1425,6 +1425,7 @@ static int batch_upload_cache_guarded(gomel_batch* b, gomel_cache* c, const int6
     if (!b || !c || !slots) return GOMEL_ERR_NULL;
     gomel_handle* h = b->h;
     if ((uintptr_t)slots % 8 || b->direct || b->io32 || c->l.K != h->cfg.num_mels || c->device != h->device || b->total_frames > (int64_t)kMaxRows) return GOMEL_ERR_BAD_CONFIG;
+    if (stream_capturing(caller)) return GOMEL_ERR_BAD_CONFIG;   // follow() would pull the handle's stream into the capture
     std::lock_guard<std::mutex> lk(h->mu);
     DeviceGuard dg(h->device); HIPCHK(dg.err);
     const int kind = memory_kind(slots, h->device);
@@ -1944,6 +1945,7 @@ static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* con
         for (size_t f = 0; f < F[u]; f++) fx[foff[u] + f] = (int64_t)(woff[u] + f * (size_t)hop);
     if (into && into->n != tot_f) return GOMEL_ERR_BAD_LENGTH;
     if (into && ((uintptr_t)into->slots % 8 || into->c->l.K != K || into->c->device != h->device || tot_f > kMaxRows)) return GOMEL_ERR_BAD_CONFIG;
+    if (into && stream_capturing(into->caller)) return GOMEL_ERR_BAD_CONFIG;
     std::lock_guard<std::mutex> lk(h->mu);
     DeviceGuard dg(h->device); HIPCHK(dg.err);
     const int slots_kind = into ? memory_kind(into->slots, h->device) : 1;

@@ -315,11 +315,11 @@ int gomel_cache_bad_slots(gomel_cache* c, uint64_t* count);
 /* gomel_batch_upload (of a batch of gomel_batch_create) with the spectrograms taken from a cache of the same NumMels and device: slots[f] for the batch's frames in
  * order (host or device memory; every one a slot of the cache: padding and slots >= n_slots are refused with GOMEL_ERR_TABLE_RANGE,
  * and the batch then has to be uploaded again).  Work queued on `stream` before the call is seen.  Returns when the batch is uploaded,
- * as gomel_batch_upload does. */
+ * as gomel_batch_upload does; not while `stream` is being captured (GOMEL_ERR_BAD_CONFIG). */
 int gomel_batch_upload_cache(gomel_batch* b, gomel_cache* c, const int64_t* slots, const double* const* x0, const uint64_t* seeds, void* stream);
 /* gomel_to_mel_batch into a cache: the log-mel frames never leave the device.  n_slots_given = frames expected (must equal the sum of
  * gomel_to_mel_pairs / NumMels over the utterances), slots as above, in the order of the utterances.  Returns when they are written;
- * work queued on `stream` before the call is waited for. */
+ * work queued on `stream` before the call is waited for; not while `stream` is being captured (GOMEL_ERR_BAD_CONFIG). */
 int gomel_to_mel_cache(gomel_handle* h, size_t n_utt, const double* const* wave, const size_t* n_samples, gomel_cache* c,
                        const int64_t* slots, size_t n_slots_given, void* stream);
 

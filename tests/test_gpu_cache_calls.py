@@ -277,3 +277,59 @@ def _dropped_tensors_child(rep):
 def test_tensors_dropped_while_a_named_stream_uses_them():
     import _children
     assert _children.run_child(_dropped_tensors_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ calls that wait, in a capture
+def _capture_child(rep):
+    import torch
+    import gomel_amd
+    torch.zeros(1, device="cuda")
+    K = 16
+    e = engine(K, Device=0, GriffinLimIterations=2)
+    c = e.cache(64)
+    x, out = torch.randn(40, K, 2, device="cuda"), torch.empty(40, K, 2, device="cuda")
+    c.write(x)
+    at = torch.arange(5, 25, device="cuda")
+    wave = np.random.default_rng(0).normal(size=30000)
+    n = len(e.to_mel_batch([wave])[0]) // K
+    b = gomel_amd.Batch(e, [20 * K])
+    want = e.from_cache(c, [at], seeds=[3])
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.write(x)
+        named = torch.cuda.current_stream()
+        for call in (lambda: e.from_cache(c, [at], seeds=[3]), lambda: e.from_cache(c, [list(range(5, 25))], seeds=[3]),
+                     lambda: e.from_cache(c, [list(range(5, 25))], seeds=[3], stream=named.cuda_stream),
+                     lambda: b.upload_cache(c, at), lambda: b.upload_cache(c, np.arange(20)), lambda: b.upload_cache(c, at, stream=named),
+                     lambda: e.to_mel_cache([wave], c, list(range(n))), lambda: e.to_mel_cache([wave], c, list(range(n)), stream=named)):
+            with pytest.raises(gomel_amd.GomelError) as err:
+                call()
+            assert err.value.status == 1
+        c.read(out)
+    for i in range(3):
+        xi = torch.randn_like(x)
+        x.copy_(xi)
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        c.write(xi, values=out)                          # the program's own work between the replays
+        assert torch.equal(got, out), i
+        assert e.to_mel_cache([wave], c, list(range(n))) == [n]
+        b.upload_cache(c, at, None, [3])
+    with torch.no_grad():
+        x.copy_(torch.randn_like(x))
+    c.write(x, values=out)
+    assert not np.array_equal(e.from_cache(c, [at], seeds=[3])[0], want[0])
+    b.close()
+    c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_calls_that_wait_are_refused_in_a_capture_which_goes_on():
+    import _children
+    assert _children.run_child(_capture_child)["ok"]
