@@ -718,7 +718,7 @@ struct OnDevice {   // the calling thread's device switched to `dev` and back
     }
     ~OnDevice() { if (prev >= 0) (void)hipSetDevice(prev); }
 };
-int hip_failed(hipError_t e) { g_last_hip = (int)e; (void)hipGetLastError(); return GOMEL_ERR_HIP; }
+int hip_failed(hipError_t e) { set_last_hip((int)e); (void)hipGetLastError(); return GOMEL_ERR_HIP; }
 #define CHK(expr) do { const hipError_t e_ = (expr); if (e_ != hipSuccess) return hip_failed(e_); } while (0)
 
 hipError_t dropout_device(int type, const void* x, size_t xs, void* y, size_t ys, size_t rows, size_t cols, const DropRule& d, uint64_t seed, uint64_t offset, hipStream_t s) {
@@ -939,6 +939,9 @@ hipError_t cache_read_device(gomel_cache* c, int type, void* y, size_t ys, size_
 
 // ------------------------------------------------------------------------------------------------ C ABI
 extern "C" {
+
+// Diagnostics (not in the header; the tests reach it by name): what every call here returns when the runtime failed with `e`.
+int gomel_debug_hip_failed(int e) { return hip_failed((hipError_t)e); }
 
 int gomel_cache_create(gomel_handle* h, size_t n_slots, int bits, int group_bands, gomel_cache** out) {
     GOMEL_TRY return cache_create(h, n_slots, bits, group_bands, out); GOMEL_CATCH

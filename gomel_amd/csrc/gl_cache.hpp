@@ -19,8 +19,6 @@ struct gomel_cache {
     size_t stage_bytes = 0;
 };
 
-extern thread_local int g_last_hip GL_HIDDEN;   // gomel_last_hip_error's value (gomel_hip.hip)
-
 // defined in gl_cache.hip: device-side halves for callers that hold device pointers already.  `n` <= kMaxRows, arguments checked.
 GL_HIDDEN hipError_t cache_write_device(gomel_cache* c, int type, const void* x, size_t xs, size_t n, const int64_t* slots, size_t first, void* y, size_t ys, hipStream_t s);
 // strict: negative slots count as bad too; `bad` receives the count instead of the cache's counter
@@ -32,6 +30,9 @@ GL_HIDDEN int memory_kind(const void* p, int device);
 GL_HIDDEN bool stream_capturing(hipStream_t s);
 
 // defined in gomel_hip.hip
+// gomel_last_hip_error's value, by a function: a thread_local variable that another file declares is reached through its initialiser's
+// address, which a hidden one without an initialiser has none of
+GL_HIDDEN void set_last_hip(int e);
 GL_HIDDEN int handle_device(const gomel_handle* h);
 GL_HIDDEN int handle_num_mels(const gomel_handle* h);
 GL_HIDDEN hipStream_t handle_stream(const gomel_handle* h);

@@ -23,7 +23,8 @@
 #include "gl_kernels.hpp"
 
 // =============================================================================================== host side
-thread_local int g_last_hip = 0;
+static thread_local int g_last_hip = 0;
+void set_last_hip(int e) { g_last_hip = e; }
 #define HIPCHK(expr)                                         \
     do {                                                     \
         hipError_t e_ = (expr);                              \

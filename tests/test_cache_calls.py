@@ -1,6 +1,7 @@
 """CPU tests of how the Python side of the spectrogram cache and dropout makes its calls: the stream it picks, what it refuses, what it
 counts.  The library is replaced by a recorder; nothing here touches a device."""
 import ctypes
+import os
 import sys
 import types
 
@@ -157,3 +158,13 @@ def _tracked_tensors_child(rep):
 def test_tensors_that_autograd_follows_are_not_written_behind_its_back():
     import _children
     assert _children.run_child(_tracked_tensors_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ a runtime call that fails
+def test_a_runtime_error_is_a_status():
+    """What the cache's and dropout's calls do when the runtime fails: a status and the error's number -- in a child, which must live."""
+    import subprocess
+    code = ("import ctypes\nfrom gomel_amd import _lib\nL = _lib.lib()\nf = L.gomel_debug_hip_failed\nf.restype, f.argtypes = ctypes.c_int, [ctypes.c_int]\n"
+            "assert f(2) == 8 and L.gomel_last_hip_error() == 2\nassert f(719) == 8 and L.gomel_last_hip_error() == 719\nprint('lives')\n")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0 and r.stdout == "lives\n", (r.returncode, r.stderr)

@@ -333,3 +333,19 @@ def _capture_child(rep):
 def test_calls_that_wait_are_refused_in_a_capture_which_goes_on():
     import _children
     assert _children.run_child(_capture_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ a runtime call that fails
+def test_a_cache_that_does_not_fit_the_memory():
+    import gomel_amd
+    from gomel_amd import _lib
+    e = engine(80)
+    with pytest.raises(gomel_amd.GomelError) as err:
+        e.cache(2 ** 36)                                 # 12 TB
+    assert err.value.status == 8 and _lib.lib().gomel_last_hip_error() == 2
+    c = e.cache(4)                                       # and everything goes on
+    x = frames(4, 80, 1).astype(np.float32)
+    c.write(x)
+    assert np.any(c.read(np.empty_like(x)) != 0)
+    c.close()
+    e.close()
