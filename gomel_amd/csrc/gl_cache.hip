@@ -694,9 +694,11 @@ constexpr size_t kStreamBytes = (size_t)64 << 20, kStreamInBytes = (size_t)128 <
 // A launch has fewer than 2^32 lanes: grids of more blocks go out in parts, a block's index counted on through them (`block0`).  Launches
 // report their own status: hipGetLastError could hand back somebody else's.
 constexpr size_t kBlocks = (size_t)1 << 22;
+thread_local int g_fail_launch = 0;   // gomel_debug_fail_launch
 template <class Args> hipError_t launch(void (*k)(Args), size_t blocks, unsigned block, hipStream_t s, Args& a) {
     hipError_t e = hipSuccess;
     for (size_t b = 0; b < blocks && e == hipSuccess; b += kBlocks) {
+        if (g_fail_launch && --g_fail_launch == 0) return hipErrorLaunchFailure;
         a.block0 = (int64_t)b;
         void* p[] = {&a};
         e = hipLaunchKernel((const void*)k, dim3((unsigned)std::min(kBlocks, blocks - b)), dim3(block), p, 0, s);
@@ -914,12 +916,16 @@ hipError_t cache_write_device(gomel_cache* c, int type, const void* x, size_t xs
     if (e != hipSuccess) return e;
     if (!a.p.units) {
         GL_TYPES(type, e = launch(k_write_wide<T>, n, 256, s, a));
-        return e;
+    } else {
+        const size_t per = 256 >> a.p.lanes_log2, blocks = (n * (size_t)a.p.segs + per - 1) / per;
+        const int streamed = 2 * (size_t)c->l.K * n * type_bytes(type) < kStreamBytes ? 0 : n * (size_t)c->l.row_bytes < kStreamInBytes ? 1 : 2;
+        GL_TYPES(type, e = launch(write_kernel<T>(a.p.units, grouped, streamed), blocks, 256, s, a));
     }
-    const size_t per = 256 >> a.p.lanes_log2, blocks = (n * (size_t)a.p.segs + per - 1) / per;
-    const int streamed = 2 * (size_t)c->l.K * n * type_bytes(type) < kStreamBytes ? 0 : n * (size_t)c->l.row_bytes < kStreamInBytes ? 1 : 2;
-    GL_TYPES(type, e = launch(write_kernel<T>(a.p.units, grouped, streamed), blocks, 256, s, a));
-    if (claims && a.p.segs > 1 && e == hipSuccess) e = launch_claim(k_claim_clear, a.slots, a.n, c->claim, s);
+    // a write that was not launched, or not all of it, leaves claims standing: a later call's lower rows would lose to them
+    if (claims && (a.p.segs > 1 || e != hipSuccess)) {
+        const hipError_t e2 = launch_claim(k_claim_clear, a.slots, a.n, c->claim, s);
+        if (e == hipSuccess) e = e2;
+    }
     return e;
 }
 
@@ -942,6 +948,9 @@ extern "C" {
 
 // Diagnostics (not in the header; the tests reach it by name): what every call here returns when the runtime failed with `e`.
 int gomel_debug_hip_failed(int e) { return hip_failed((hipError_t)e); }
+// Diagnostics (not in the header; the tests reach it by name): the calling thread's n-th launch of a write, read or dropout kernel from now
+// on fails without being launched, as one that the runtime refuses would.  0: none.
+void gomel_debug_fail_launch(int n) { g_fail_launch = n; }
 
 int gomel_cache_create(gomel_handle* h, size_t n_slots, int bits, int group_bands, gomel_cache** out) {
     GOMEL_TRY return cache_create(h, n_slots, bits, group_bands, out); GOMEL_CATCH

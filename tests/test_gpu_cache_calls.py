@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import cache_reference as ref
-from test_gpu_cache import Dev, dev, engine, frames  # noqa: F401  (dev: the fixture)
+from test_gpu_cache import dev, engine, frames, held  # noqa: F401  (dev: the fixture)
 
 pytestmark = [pytest.mark.gpu]
 
@@ -347,5 +347,35 @@ def test_a_cache_that_does_not_fit_the_memory():
     x = frames(4, 80, 1).astype(np.float32)
     c.write(x)
     assert np.any(c.read(np.empty_like(x)) != 0)
+    c.close()
+    e.close()
+
+
+# ------------------------------------------------------------------------------------------------ a launch that fails
+@pytest.mark.parametrize("K,dtype,group,n", [(24, "float32", 8, 5000), (515, "float64", 0, 2100), (515, "float64", 32, 4200)])
+def test_a_write_that_fails_leaves_no_claim_behind(dev, K, dtype, group, n):  # noqa: F811
+    """The frames claim their slots in a launch before the write's.  When the write's fails, the next write of the same slots from other,
+    lower rows has to reach the cache: frames under one scale, in segments and block-wide."""
+    import gomel_amd
+    from gomel_amd import _lib
+    e = engine(K, Resolut=8192) if K > 700 else engine(K)
+    c = e.cache(n, 8, group)
+    x = frames(8, K, 1)
+    want = ref.stands_for(held(x, dtype), 8, group)
+    which = np.arange(n) % 8
+    src, up, down = dev.up(x[which], dtype), dev.up(np.arange(n), "int64"), dev.up(np.arange(n)[::-1], "int64")
+    fail = _lib.lib().gomel_debug_fail_launch
+    fail.restype, fail.argtypes = None, [ctypes.c_int]
+    fail(1)
+    with pytest.raises(gomel_amd.GomelError) as err:
+        c.write(src, slots=up)
+    assert err.value.status == 8
+    assert not c.read(np.empty((n, K, 2))).any()
+    c.write(src, slots=down)                             # slot n - 1 now comes from row 0: a claim of row n - 1 must not stand in its way
+    got = c.read(np.empty((n, K, 2)))[::-1]
+    for i in range(8):
+        assert ref.close(got[which == i], (np.broadcast_to(want[i], got[which == i].shape), np.abs(want[i]) + 32), "float64", 2), i
+    c.write(src, slots=up)
+    assert np.array_equal(c.read(np.empty((n, K, 2))), got)
     c.close()
     e.close()
