@@ -5,6 +5,7 @@ tensors on the engine's device (those types and bfloat16; the call queues kernel
 `DevicePointer`s.  There is no CPU fallback."""
 import ctypes
 import sys
+from operator import index as _index     # any integer's value: Python's, numpy's, a torch scalar's
 
 import numpy as np
 
@@ -13,6 +14,7 @@ from ._lib import GomelError, check
 from .mel import Batch, DevicePointer
 
 _ON_DEVICE = 0x100           # GOMEL_DEVICE_MEMORY: nothing of the call is in host memory
+_U64 = 0xFFFFFFFFFFFFFFFF
 _TYPES = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}
 _torch = _forward_ad = None  # the modules torch and torch.autograd.forward_ad, once a tensor has been seen
 _increment_version = None    # torch.autograd.graph.increment_version of an iterable of tensors
@@ -274,7 +276,7 @@ class Cache:
             t |= _ON_DEVICE
         else:
             on = _device_of(on, dev, sdev)
-        rc = self._read(self._c, t, ptr, stride, n, sp, first, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on, self.device))
+        rc = self._read(self._c, t, ptr, stride, n, sp, first, p, _index(seed) & _U64, _index(offset) & _U64, _stream(stream, on, self.device))
         _written(out)
         if stream is not None:
             _used_on(stream, out, slots)
@@ -370,7 +372,7 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
     if out is not None and _Tensor is not None and isinstance(x, _Tensor) and isinstance(out, _Tensor) and x.is_contiguous() and out.is_contiguous() and x.shape == out.shape and x.dtype == out.dtype:
         t, n = _torch_types.get(x.dtype), x.numel()                       # two dense tensors: nothing to work out
         if t is not None and n and device == x.get_device() == out.get_device():
-            rc = fn(engine._h, t | _ON_DEVICE, x.data_ptr(), n, out.data_ptr(), n, 1, n, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
+            rc = fn(engine._h, t | _ON_DEVICE, x.data_ptr(), n, out.data_ptr(), n, 1, n, p, _index(seed) & _U64, _index(offset) & _U64,
                     _raw_stream(device) if stream is None else _stream(stream, device, device))
             _increment_version((out,))
             if stream is not None:
@@ -396,7 +398,7 @@ def _dropout(fn, where, engine, x, p, seed, offset, out, stream):
     on = _device_of(device, dev, odev)
     if on == device and dev is not None and odev is not None:
         t |= _ON_DEVICE
-    rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, _stream(stream, on, device))
+    rc = fn(engine._h, t, ptr, xs, optr, os_, rows, cols, p, _index(seed) & _U64, _index(offset) & _U64, _stream(stream, on, device))
     _written(out)
     if stream is not None:
         _used_on(stream, x, out)

@@ -168,3 +168,23 @@ def test_a_runtime_error_is_a_status():
             "assert f(2) == 8 and L.gomel_last_hip_error() == 2\nassert f(719) == 8 and L.gomel_last_hip_error() == 719\nprint('lives')\n")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0 and r.stdout == "lives\n", (r.returncode, r.stderr)
+
+
+# ------------------------------------------------------------------------------------------------ integers of every kind
+def test_seeds_and_offsets_are_any_integers():
+    from gomel_amd import cache
+    c, seen = _recording()
+    x = np.zeros((2, 4, 2), np.float32)
+    for v, want in ((5, 5), (-1, 2 ** 64 - 1), (2 ** 64 + 3, 3), (np.int64(7), 7), (np.int64(-2), 2 ** 64 - 2), (np.uint32(9), 9), (np.int8(-1), 2 ** 64 - 1),
+                    (np.uint64(2 ** 64 - 1), 2 ** 64 - 1), (np.random.default_rng(1).integers(0, 2 ** 40), None), (True, 1)):
+        want = int(v) if want is None else want
+        del seen[:]
+        c.read(x, p=0.5, seed=v, offset=v)
+        cache._dropout(lambda *a: seen.append(a) or 0, "here", _Engine, x, 0.5, v, v, None, None)
+        for a in seen:
+            assert a[-3:-1] == (want, want) and all(type(k) is int for k in a[-3:-1]), v
+    for v in (1.0, "1", None, np.float64(2)):
+        with pytest.raises(TypeError):
+            c.read(x, p=0.5, seed=v)
+        with pytest.raises(TypeError):
+            c.read(x, p=0.5, offset=v)
