@@ -15,6 +15,7 @@ from .mel import Batch, DevicePointer
 
 _ON_DEVICE = 0x100           # GOMEL_DEVICE_MEMORY: nothing of the call is in host memory
 _U64 = 0xFFFFFFFFFFFFFFFF
+_FAR = 2 ** 63               # stands for every number of slots from there on: the library refuses it
 _TYPES = {"float64": 0, "float32": 1, "float16": 2, "bfloat16": 3}
 _torch = _forward_ad = None  # the modules torch and torch.autograd.forward_ad, once a tensor has been seen
 _increment_version = None    # torch.autograd.graph.increment_version of an iterable of tensors
@@ -217,6 +218,12 @@ def _slots(slots, n, what="slots"):
     return (a.ctypes.data if n else 0), a, None
 
 
+def _far(first):
+    if first < 0:
+        raise ValueError("first is negative")
+    return _FAR
+
+
 class Cache:
     """gomel_cache: `n_slots` slots of one quantised frame ([NumMels][2] values) in the device's memory.  `bits` 8 or 4 per value; `group`
     bands share a minimum and a step (0 = the whole frame, or 8, 16, 32, 64).  Pages and their tables are the caller's: `slots` names one
@@ -229,8 +236,9 @@ class Cache:
         if self.n_slots < 0:
             raise ValueError("n_slots is negative")
         L = _lib.lib()
-        self.frame_bytes = L.gomel_cache_frame_bytes(ctypes.byref(engine.cfg), self.bits, self.group)
-        check(L.gomel_cache_create(engine._h, self.n_slots, self.bits, self.group, ctypes.byref(self._c)), "gomel_cache_create")
+        held = min(self.n_slots, _FAR), *(v if abs(v) < 2 ** 31 else -1 for v in (self.bits, self.group))    # (ctypes would cut the rest off)
+        self.frame_bytes = L.gomel_cache_frame_bytes(ctypes.byref(engine.cfg), *held[1:])
+        check(L.gomel_cache_create(engine._h, *held, ctypes.byref(self._c)), "gomel_cache_create")
         self._write, self._read = L.gomel_cache_write, L.gomel_cache_read
 
     def write(self, frames, slots=None, first=0, values=None, stream=None):
@@ -248,8 +256,8 @@ class Cache:
             vp, vt, vs, vn, vdev = _rows(values, cols, "values", write=True)
             if vt != t or vn != n:
                 raise ValueError("values: the frames' type and number of frames are needed")
-        if first < 0:
-            raise ValueError("first is negative")
+        if not 0 <= first < _FAR:
+            first = _far(first)
         on = self.device
         if dev == on and (values is None or vdev == on) and (slots is None or sdev == on):
             t |= _ON_DEVICE
@@ -269,8 +277,8 @@ class Cache:
         _output(out, "out")
         ptr, t, stride, n, dev = _rows(out, 2 * self.num_mels, "out", write=True)
         sp, keep, sdev = (0, None, None) if slots is None else _slots(slots, n)
-        if first < 0:
-            raise ValueError("first is negative")
+        if not 0 <= first < _FAR:
+            first = _far(first)
         on = self.device
         if dev == on and (slots is None or sdev == on):
             t |= _ON_DEVICE

@@ -188,3 +188,30 @@ def test_seeds_and_offsets_are_any_integers():
             c.read(x, p=0.5, seed=v)
         with pytest.raises(TypeError):
             c.read(x, p=0.5, offset=v)
+
+
+def test_numbers_beyond_the_librarys_are_not_cut_off(monkeypatch):
+    import gomel_amd
+    from gomel_amd import _lib, cache
+    c, seen = _recording()
+    x = np.zeros((2, 4, 2), np.float32)
+    for first in (2 ** 63, 2 ** 64, 2 ** 64 + 3, 2 ** 200):                  # (2 ** 64 + 3 was slot 3)
+        del seen[:]
+        c.write(x, first=first)
+        c.read(x, first=first)
+        assert [a[6] for a in seen] == [2 ** 63] * 2                         # no cache has it: the library refuses
+    c.write(x, first=np.int64(3))
+    assert seen[-1][6] == 3
+    with pytest.raises(ValueError):
+        c.read(x, first=-2 ** 70)
+    L, made = _lib.lib(), []
+    cfg = _lib.GomelConfig()
+    L.gomel_default_config(ctypes.byref(cfg))
+    eng = types.SimpleNamespace(cfg=cfg, _h=None)
+    monkeypatch.setattr(cache._lib, "lib", lambda: types.SimpleNamespace(gomel_cache_frame_bytes=L.gomel_cache_frame_bytes, gomel_cache_write=None, gomel_cache_read=None,
+                                                                         gomel_cache_create=lambda h, n, b, g, out: made.append((n, b, g)) or 0,
+                                                                         gomel_cache_destroy=lambda c: 0))
+    for args, want in (((2 ** 64 + 4, 8, 0), (2 ** 63, 8, 0)), ((4, 2 ** 32 + 8, 0), (4, -1, 0)), ((4, 8, 2 ** 32), (4, 8, -1)), ((4, 8 - 2 ** 32, 16), (4, -1, 16)),
+                       ((5, 4, 64), (5, 4, 64))):
+        k = gomel_amd.Cache(eng, *args)
+        assert made.pop() == want and (k.frame_bytes > 0) == (want[1] > 0 and want[2] >= 0)
