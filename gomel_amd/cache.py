@@ -196,6 +196,15 @@ def _written(a):
         _increment_version((a,))
 
 
+def _host_slots(slots, what):
+    a = np.asarray(slots)
+    if a.dtype.kind not in "iu" and a.size:
+        raise ValueError("%s: integers are needed, not %s" % (what, a.dtype))
+    if a.dtype.kind == "u" and a.size and int(a.max()) > 2 ** 63 - 1:
+        raise ValueError("%s: beyond int64" % what)
+    return np.ascontiguousarray(a, dtype=np.int64).reshape(-1)
+
+
 def _slots(slots, n, what="slots"):
     """(address, the array that has to stay alive, device) of one int64 per frame."""
     if _is_tensor(slots) if _Tensor is None else isinstance(slots, _Tensor):
@@ -207,12 +216,7 @@ def _slots(slots, n, what="slots"):
         if slots.dtype != "int64" or slots.numel() != n:
             raise ValueError("%s: a DevicePointer of %d int64 is needed" % (what, n))
         return slots.data_ptr(), slots, None
-    a = np.asarray(slots)
-    if a.dtype.kind not in "iu" and a.size:
-        raise ValueError("%s: integers are needed, not %s" % (what, a.dtype))
-    if a.dtype.kind == "u" and a.size and int(a.max()) > 2 ** 63 - 1:
-        raise ValueError("%s: beyond int64" % what)
-    a = np.ascontiguousarray(a, dtype=np.int64).reshape(-1)
+    a = _host_slots(slots, what)
     if a.size != n:
         raise ValueError("%s: one slot per frame is needed (%d frames, %d slots)" % (what, n, a.size))
     return (a.ctypes.data if n else 0), a, None
@@ -319,20 +323,31 @@ def batch_upload_cache(batch, cache, slots, x0s=None, seeds=None, stream=None):
     del xs, keep
 
 
+def _joined(slots, stream, engine_device):
+    """(all utterances' slots as one array, how many each has)"""
+    tensors = sum(_is_tensor(s) for s in slots)
+    if not tensors and len(slots) == 1 and isinstance(slots[0], DevicePointer):
+        return slots[0], [slots[0].numel()]
+    if not tensors and not any(isinstance(s, DevicePointer) for s in slots):
+        arrays = [_host_slots(s, "slots") for s in slots]
+        return np.concatenate(arrays), [a.size for a in arrays]
+    if tensors != len(slots):                    # (DevicePointers of several utterances: Batch.upload_cache takes them as one)
+        raise ValueError("slots: of several utterances, either all in host memory or all as int64 CUDA tensors")
+    if any(s.dtype != _int64 or not s.is_cuda for s in slots):
+        raise ValueError("slots: int64 CUDA tensors are needed (numpy arrays are taken from host memory)")
+    on = _device_of(engine_device, *[s.get_device() for s in slots])
+    # in the order of the call's stream: there the slots are ready, and there they are read
+    with _torch.cuda.stream(_torch.cuda.current_stream(on) if stream is None else _as_stream(stream, on)):
+        return _torch.cat([s.reshape(-1) for s in slots]), [s.numel() for s in slots]
+
+
 def from_cache(engine, cache, slots, x0s=None, seeds=None, stream=None):
-    counts = [int(s.numel()) if hasattr(s, "numel") else len(s) for s in slots]
-    if not counts:
+    slots = list(slots)
+    if not slots:
         return []
     if _capturing(stream, cache.device):         # as gomel_batch_upload_cache, before a batch is allocated
         raise GomelError(1, "from_cache")
-    tensors = [s for s in slots if _is_tensor(s)]
-    if tensors and stream is not None and tensors[0].is_cuda:   # joined in the order of the call's stream: there the slots are ready, and there they are read
-        with _torch.cuda.stream(_as_stream(stream, tensors[0].device)):
-            flat = _torch.cat([s.reshape(-1) for s in slots])
-    elif tensors:
-        flat = _torch.cat([s.reshape(-1) for s in slots])
-    else:
-        flat = np.concatenate([np.asarray(s, dtype=np.int64).reshape(-1) for s in slots])
+    flat, counts = _joined(slots, stream, cache.device)
     b = Batch(engine, [c * engine.cfg.num_mels for c in counts])
     try:
         b.upload_cache(cache, flat, x0s, seeds, stream)

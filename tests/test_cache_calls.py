@@ -215,3 +215,31 @@ def test_numbers_beyond_the_librarys_are_not_cut_off(monkeypatch):
                        ((5, 4, 64), (5, 4, 64))):
         k = gomel_amd.Cache(eng, *args)
         assert made.pop() == want and (k.frame_bytes > 0) == (want[1] > 0 and want[2] >= 0)
+
+
+# ------------------------------------------------------------------------------------------------ the slots of several utterances
+def test_slots_of_several_utterances():
+    from gomel_amd import DevicePointer
+    from gomel_amd.cache import _joined
+    for slots in ([[1, 2, 3], [4, 5]], [np.array([1, 2, 3], np.int32), (4, 5)], [np.array([[1], [2], [3]]), np.uint64([4, 5])]):
+        flat, counts = _joined(slots, None, 0)
+        assert flat.dtype == np.int64 and flat.tolist() == [1, 2, 3, 4, 5] and counts == [3, 2]
+    p = DevicePointer(64, 7, "int64")
+    assert _joined([p], None, 0) == (p, [7])
+    for slots in ([[1.0, 2.5]], [np.array([1.0])], [[1], [2 ** 63]], [["1"]], [p, p], [p, [1]], [np.array([2 ** 63], np.uint64)]):
+        with pytest.raises(ValueError):
+            _joined(slots, None, 0)
+
+
+def test_from_cache_refuses_before_it_allocates_a_batch(monkeypatch):
+    from gomel_amd import DevicePointer, cache
+    c = _cache()
+
+    def batch(*a):
+        raise AssertionError("a batch was allocated")
+    monkeypatch.setattr(cache, "Batch", batch)
+    assert cache.from_cache(_Engine, c, []) == [] and cache.from_cache(_Engine, c, iter(())) == []
+    p = DevicePointer(64, 7, "int64")
+    for slots in ([[1.5]], [p, p], [[1], p], iter([[1], [0.5]])):
+        with pytest.raises(ValueError):
+            cache.from_cache(_Engine, c, slots)

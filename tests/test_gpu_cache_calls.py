@@ -379,3 +379,43 @@ def test_a_write_that_fails_leaves_no_claim_behind(dev, K, dtype, group, n):  # 
     assert np.array_equal(c.read(np.empty((n, K, 2))), got)
     c.close()
     e.close()
+
+
+# ------------------------------------------------------------------------------------------------ the slots of several utterances
+def test_slots_of_every_kind_into_from_mel(dev):  # noqa: F811
+    K = 16
+    e = engine(K, GriffinLimIterations=2)
+    c = e.cache(64)
+    c.write(frames(64, K, 2))
+    want = e.from_cache(c, [np.arange(8, 20), np.arange(30, 45)], seeds=[1, 2])
+    for slots in ([list(range(8, 20)), tuple(range(30, 45))], [np.arange(8, 20)[:, None], np.arange(30, 45, dtype=np.uint8)], iter([range(8, 20), range(30, 45)])):
+        got = e.from_cache(c, slots, seeds=[1, 2])
+        assert all(np.array_equal(g, w) for g, w in zip(got, want)) and len(got) == 2
+    assert np.array_equal(e.from_cache(c, [dev.up(np.arange(8, 20), "int64")], seeds=[1])[0], want[0])
+    c.close()
+    e.close()
+
+
+def _slot_tensors_child(rep):
+    import torch
+    torch.zeros(1, device="cuda")
+    e = engine(16, Device=0, GriffinLimIterations=2)
+    c = e.cache(64)
+    a, b = torch.arange(8, 20, device="cuda"), torch.arange(30, 45, device="cuda")
+    c.write(torch.randn(64, 16, 2, device="cuda"))
+    want = e.from_cache(c, [a, b], seeds=[1, 2])
+    got = e.from_cache(c, [a.view(3, 4), torch.arange(30, 60, device="cuda")[:30].view(15, 2)[:, 0] * 0 + b], seeds=[1, 2])
+    assert all(np.array_equal(g, w) for g, w in zip(got, want))
+    for bad in ([a, [30, 31]], [a, b.int()], [a.float(), b], [a, b.cpu()], [a.cpu()], [a > 3]):
+        with pytest.raises(ValueError):
+            e.from_cache(c, bad)
+    c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_slot_tensors_into_from_mel():
+    import _children
+    assert _children.run_child(_slot_tensors_child)["ok"]
