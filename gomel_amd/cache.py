@@ -228,6 +228,19 @@ def _far(first):
     return _FAR
 
 
+_left = []                   # (cache, device) of those closed or collected while torch's current stream was being captured
+
+
+def _destroy_left(device):
+    if _left and not _capturing(None, device):
+        for k in [k for k in _left if not _capturing(None, k[1])]:
+            try:
+                _left.remove(k)
+            except ValueError:               # another thread has it
+                continue
+            _lib.lib().gomel_cache_destroy(k[0])
+
+
 class Cache:
     """gomel_cache: `n_slots` slots of one quantised frame ([NumMels][2] values) in the device's memory.  `bits` 8 or 4 per value; `group`
     bands share a minimum and a step (0 = the whole frame, or 8, 16, 32, 64).  Pages and their tables are the caller's: `slots` names one
@@ -239,6 +252,7 @@ class Cache:
         self.device = int(engine.cfg.device)
         if self.n_slots < 0:
             raise ValueError("n_slots is negative")
+        _destroy_left(self.device)
         L = _lib.lib()
         held = min(self.n_slots, _FAR), *(v if abs(v) < 2 ** 31 else -1 for v in (self.bits, self.group))    # (ctypes would cut the rest off)
         self.frame_bytes = L.gomel_cache_frame_bytes(ctypes.byref(engine.cfg), *held[1:])
@@ -267,6 +281,8 @@ class Cache:
             t |= _ON_DEVICE
         else:
             on = _device_of(on, dev, vdev, sdev)
+        if _left:
+            _destroy_left(self.device)
         rc = self._write(self._c, t, ptr, stride, n, sp, first, vp, vs, _stream(stream, on, self.device))
         _written(values)
         if stream is not None:
@@ -288,6 +304,8 @@ class Cache:
             t |= _ON_DEVICE
         else:
             on = _device_of(on, dev, sdev)
+        if _left:
+            _destroy_left(self.device)
         rc = self._read(self._c, t, ptr, stride, n, sp, first, p, _index(seed) & _U64, _index(offset) & _U64, _stream(stream, on, self.device))
         _written(out)
         if stream is not None:
@@ -303,9 +321,15 @@ class Cache:
         return n.value
 
     def close(self):
+        """Gives the memory back -- in a capture (gomel_cache_destroy waits for the device, which would end it) when the next call of any
+        cache is made outside one."""
         if self._c:
             c, self._c = self._c, ctypes.c_void_p()
-            check(_lib.lib().gomel_cache_destroy(c), "gomel_cache_destroy")
+            if _capturing(None, self.device):
+                _left.append((c, self.device))
+            else:
+                _destroy_left(self.device)
+                check(_lib.lib().gomel_cache_destroy(c), "gomel_cache_destroy")
 
     def __del__(self):
         try:

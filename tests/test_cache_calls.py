@@ -243,3 +243,37 @@ def test_from_cache_refuses_before_it_allocates_a_batch(monkeypatch):
     for slots in ([[1.5]], [p, p], [[1], p], iter([[1], [0.5]])):
         with pytest.raises(ValueError):
             cache.from_cache(_Engine, c, slots)
+
+
+# ------------------------------------------------------------------------------------------------ closed or collected in a capture
+def test_a_cache_dropped_in_a_capture_is_destroyed_behind_it(monkeypatch):
+    import gc
+    from gomel_amd import cache
+    gone, busy = [], [True]
+    monkeypatch.setattr(cache, "_left", [])
+    monkeypatch.setattr(cache, "_capturing", lambda stream, device: busy[0])
+    monkeypatch.setattr(cache._lib, "lib", lambda: types.SimpleNamespace(gomel_cache_destroy=lambda c: gone.append(c.value) or 0))
+
+    def made(v):
+        c, _ = _recording()
+        c._c = ctypes.c_void_p(v)
+        return c
+    a, b, live = made(11), made(12), made(13)
+    x = np.zeros((1, 4, 2), np.float32)
+    a.close()
+    a.close()
+    del b
+    gc.collect()
+    live.write(x)
+    live.read(x)
+    assert gone == []                                    # the capture goes on
+    busy[0] = False
+    live.read(x)
+    assert sorted(gone) == [11, 12]
+    made(14).close()
+    busy[0] = True
+    made(15).close()
+    assert sorted(gone) == [11, 12, 14]
+    busy[0] = False
+    live.close()
+    assert sorted(gone) == [11, 12, 13, 14, 15]

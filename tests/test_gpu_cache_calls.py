@@ -419,3 +419,47 @@ def _slot_tensors_child(rep):
 def test_slot_tensors_into_from_mel():
     import _children
     assert _children.run_child(_slot_tensors_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ closed or collected in a capture
+def _dropped_in_a_capture_child(rep):
+    import gc
+    import torch
+    torch.zeros(1, device="cuda")
+    K = 16
+    e = engine(K, Device=0)
+    c = e.cache(64)
+    x, out = torch.randn(64, K, 2, device="cuda"), torch.empty(64, K, 2, device="cuda")
+    free0 = torch.cuda.mem_get_info()[0]
+    big, other = e.cache(2 ** 26), e.cache(2 ** 25)      # 3.5 and 1.7 GB
+    held = [big]
+    held.append(held)                                    # a cycle: the collector finds it
+    c.write(x)
+    torch.cuda.synchronize()
+    assert free0 - torch.cuda.mem_get_info()[0] > 4 << 30
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.write(x)
+        del big, held
+        gc.collect()
+        other.close()
+        c.read(out)
+    for i in range(3):
+        x.copy_(torch.randn_like(x))
+        g.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        c.write(x, values=out)
+        assert torch.equal(got, out), i
+    torch.cuda.synchronize()
+    assert free0 - torch.cuda.mem_get_info()[0] < 1 << 30
+    c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_caches_dropped_in_a_capture_leave_it_alone():
+    import _children
+    assert _children.run_child(_dropped_in_a_capture_child)["ok"]
