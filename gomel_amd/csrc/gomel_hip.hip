@@ -672,6 +672,11 @@ static int batch_run_impl(gomel_batch* b, gomel_timing* tm);
 //     enqueued while persistent launches are in flight first makes its stream wait for them (hipStreamWaitEvent: <= 0.6 ms of
 //     device-side ordering, nothing blocks on the host).  The gate's mutex is held while a persistent launch is being enqueued
 //     (~0.1 ms), so that "nothing else in flight" still holds when its kernel reaches the queue.
+// Outside the gate, like another process: what a caller queues on streams of its own, the cache's and dropout's calls (gl_cache.hip)
+// included.  An event per call would cost as much as the smaller calls take, a wait for a persistent launch would hold a frame's write up
+// by a whole utterance, and neither reaches a replayed graph.  Their kernels end by themselves and most take microseconds, far below the
+// 20 ms limit; where a queue full of them still keeps a workgroup waiting longer, the launch gives up and the run is done again through
+// the per-iteration kernels (same bits).
 struct HipEvOps {
     typedef hipEvent_t Event;
     static int query(hipEvent_t ev) {
@@ -1435,6 +1440,7 @@ static int batch_upload_cache_guarded(gomel_batch* b, gomel_cache* c, const int6
     if (!kind)
         for (size_t f = 0; f < n; f++) if (slots[f] < 0 || (uint64_t)slots[f] >= c->n_slots) return GOMEL_ERR_TABLE_RANGE;
     b->uploaded = false;
+    GateOrdinary gate_o;   // the read below is ordinary kernel work; left once it has drained
     struct Temp {   // the count of bad slots | the slots, when they come from the host
         gomel_handle* h; void* p = nullptr;
         ~Temp() { if (p) { (void)hipStreamSynchronize(h->stream); h->pool.release(p); } }
@@ -1443,6 +1449,7 @@ static int batch_upload_cache_guarded(gomel_batch* b, gomel_cache* c, const int6
     unsigned long long* bad = (unsigned long long*)tmp.p;
     const int64_t* at = slots;
     HIPCHK(follow(h->stream, caller));
+    gate_o.enter(h, h->stream);
     HIPCHK(hipMemsetAsync(bad, 0, 8, h->stream));
     if (!kind) {
         at = (const int64_t*)((char*)tmp.p + 256);
@@ -1453,6 +1460,7 @@ static int batch_upload_cache_guarded(gomel_batch* b, gomel_cache* c, const int6
     unsigned long long count = 0;
     HIPCHK(hipMemcpyAsync(&count, bad, 8, hipMemcpyDeviceToHost, h->stream));
     HIPCHK(hipStreamSynchronize(h->stream));
+    gate_o.leave(nullptr, nullptr);
     if (count) return GOMEL_ERR_TABLE_RANGE;
     return batch_upload_impl(b, nullptr, (const void* const*)x0, seeds, true, true, h->stream);
 }

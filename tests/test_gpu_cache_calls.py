@@ -463,3 +463,32 @@ def _dropped_in_a_capture_child(rep):
 def test_caches_dropped_in_a_capture_leave_it_alone():
     import _children
     assert _children.run_child(_dropped_in_a_capture_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ beside a persistent launch
+def test_from_mel_out_of_the_cache_waits_for_a_persistent_launch():
+    """The read of upload_cache is ordinary kernel work: it goes behind a persistent run of another engine, not beside it."""
+    import time
+    import gomel_amd
+    K = 80
+    one = engine(K, Resolut=1024, Window=256, MelFmax=8000, GriffinLimIterations=4000)
+    one.set_path(3)                                      # persistent
+    one.set_precision(32)
+    other = engine(K)
+    c = other.cache(64)
+    c.write(frames(64, K, 1))
+    b, run = gomel_amd.Batch(other, [40 * K]), gomel_amd.Batch(one, [40 * K])
+    run.upload([frames(40, K, 3).reshape(-1, 2)], None, [1])
+    assert run.run_timed()["fast_path"] == 2
+    b.upload_cache(c, np.arange(40))
+    for _ in range(3):
+        t0 = time.perf_counter()
+        run.run()
+        b.upload_cache(c, np.arange(40))
+        t1 = time.perf_counter()
+        run.sync()
+        t2 = time.perf_counter()
+        assert t2 - t0 > 0.01, "the run is too short to show the order"
+        assert t2 - t1 < 0.2 * (t2 - t0), (t1 - t0, t2 - t0)
+    for k in (b, run, c, one, other):
+        k.close()
