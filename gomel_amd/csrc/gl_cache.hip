@@ -1006,13 +1006,13 @@ int gomel_cache_bad_slots(gomel_cache* c, uint64_t* count) {
     hipStream_t s = nullptr;
     CHK(hipStreamCreateWithFlags(&s, hipStreamNonBlocking));
     unsigned long long got = 0;
-    hipError_t e = hipMemcpyAsync(&got, c->bad, 8, hipMemcpyDeviceToHost, s);
-    if (e == hipSuccess) e = hipMemsetAsync(c->bad, 0, 8, s);
+    hipError_t e = hipMemcpyAsync(&got, c->bad, 8, hipMemcpyDeviceToHost, s);   // never set back: a running call may be counting
     const hipError_t e2 = hipStreamSynchronize(s);
     (void)hipStreamDestroy(s);
     if (e == hipSuccess) e = e2;
     if (e != hipSuccess) return hip_failed(e);
-    *count = got;
+    *count = got - c->told;
+    c->told = got;
     return GOMEL_OK;
 }
 

@@ -13,8 +13,9 @@ struct gomel_cache {
     size_t n_slots = 0;
     uint8_t* store = nullptr;           // [n_slots][row_bytes]; the next two lie behind it in the same allocation
     int32_t* claim = nullptr;           // [n_slots], -1 between calls: which frame of a large write gets the slot
-    unsigned long long* bad = nullptr;  // frames skipped because their slot was >= n_slots
-    std::mutex mu;                      // the staging buffer below
+    unsigned long long* bad = nullptr;  // frames skipped because their slot was >= n_slots, since the cache was made
+    std::mutex mu;                      // what is below
+    unsigned long long told = 0;        // of them, reported by gomel_cache_bad_slots
     void* stage = nullptr;
     size_t stage_bytes = 0;
 };

@@ -310,8 +310,8 @@ int gomel_cache_write(gomel_cache* c, int type, const void* frames, size_t strid
                       void* values, size_t values_stride, void* stream);
 int gomel_cache_read(gomel_cache* c, int type, void* frames, size_t stride, size_t n, const int64_t* slots, size_t first,
                      double p, uint64_t seed, uint64_t offset, void* stream);
-/* How many frames were skipped so far because their slot, in device memory, was >= n_slots; counts the calls whose work has finished
- * (synchronise their streams first) and starts again at zero. */
+/* How many frames were skipped since the last such call because their slot, in device memory, was >= n_slots.  Frames of calls that are
+ * still running are counted now or the next time (synchronise their streams first to have them now). */
 int gomel_cache_bad_slots(gomel_cache* c, uint64_t* count);
 /* gomel_batch_upload (of a batch of gomel_batch_create) with the spectrograms taken from a cache of the same NumMels and device: slots[f] for the batch's frames in
  * order (host or device memory; every one a slot of the cache: padding and slots >= n_slots are refused with GOMEL_ERR_TABLE_RANGE,

@@ -492,3 +492,35 @@ def test_from_mel_out_of_the_cache_waits_for_a_persistent_launch():
         assert t2 - t1 < 0.2 * (t2 - t0), (t1 - t0, t2 - t0)
     for k in (b, run, c, one, other):
         k.close()
+
+
+# ------------------------------------------------------------------------------------------------ bad slots counted beside running calls
+def _bad_slots_child(rep):
+    import torch
+    torch.zeros(1, device="cuda")
+    K, n, rounds = 16, 200_000, 400
+    e = engine(K, Device=0)
+    c = e.cache(64)
+    out = torch.zeros(n, K, 2, device="cuda")
+    at = torch.full((n,), 64, device="cuda")             # every one beyond the cache
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    told, mid = 0, 0
+    with torch.cuda.stream(side):
+        for _ in range(rounds):
+            c.read(out, slots=at)
+            told += c.bad_slots()
+            mid += 0 < told < n * rounds
+    side.synchronize()
+    told += c.bad_slots()
+    assert told == n * rounds and c.bad_slots() == 0 and mid > 0, (told, n * rounds, mid)
+    c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_no_bad_slot_is_lost_to_a_count_beside_a_running_call():
+    import _children
+    assert _children.run_child(_bad_slots_child)["ok"]
