@@ -252,6 +252,8 @@ class Cache:
         self.device = int(engine.cfg.device)
         if self.n_slots < 0:
             raise ValueError("n_slots is negative")
+        if _capturing(None, self.device):        # as the library's calls that wait: it would end the capture
+            raise GomelError(1, "gomel_cache_create")
         _destroy_left(self.device)
         L = _lib.lib()
         held = min(self.n_slots, _FAR), *(v if abs(v) < 2 ** 31 else -1 for v in (self.bits, self.group))    # (ctypes would cut the rest off)
@@ -315,7 +317,9 @@ class Cache:
         return out
 
     def bad_slots(self):
-        """Frames skipped so far because a slot in device memory was not one of the cache's (gomel_cache_bad_slots)."""
+        """Frames skipped since the last call because a slot in device memory was not one of the cache's (gomel_cache_bad_slots)."""
+        if self._c and _capturing(None, self.device):
+            raise GomelError(1, "bad_slots")
         n = ctypes.c_uint64(0)
         check(_lib.lib().gomel_cache_bad_slots(self._c, ctypes.byref(n)), "gomel_cache_bad_slots")
         return n.value

@@ -300,8 +300,9 @@ int gomel_get_precision(const gomel_handle* h, int32_t iterations, int32_t* fp64
  * generating model is to be conditioned on; a straight-through gradient of it is the identity); values may be frames itself (same stride) but must not overlap it otherwise.
  *   gomel_cache_read: dequantises n frames (fp32 arithmetic; fp64 for GOMEL_F64), rounded once to `type`.  p > 0 applies dropout
  * (below) to the values read, element index = position in the dense [n][2 * NumMels] output.
- * The cache keeps nothing of the handle (its NumMels and device are copied): either may be destroyed first.  gomel_cache_destroy waits
- * for the device's queued work: not while a stream is being captured, and not before the last replay of a graph that uses the cache. */
+ * The cache keeps nothing of the handle (its NumMels and device are copied): either may be destroyed first.  gomel_cache_create
+ * and _bad_slots wait for a stream of their own and gomel_cache_destroy for the device's queued work: none of them while a stream is being
+ * captured, and the last not before the last replay of a graph that uses the cache. */
 typedef struct gomel_cache gomel_cache;
 size_t gomel_cache_frame_bytes(const gomel_config* cfg, int bits, int group_bands); /* host only; 0 for arguments that create refuses */
 int gomel_cache_create(gomel_handle* h, size_t n_slots, int bits, int group_bands, gomel_cache** out);

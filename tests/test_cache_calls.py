@@ -277,3 +277,18 @@ def test_a_cache_dropped_in_a_capture_is_destroyed_behind_it(monkeypatch):
     busy[0] = False
     live.close()
     assert sorted(gone) == [11, 12, 13, 14, 15]
+
+
+def test_calls_that_wait_are_refused_in_a_capture(monkeypatch):
+    import gomel_amd
+    from gomel_amd import cache
+    monkeypatch.setattr(cache, "_capturing", lambda stream, device: True)
+    c, _ = _recording()
+    c._c = ctypes.c_void_p(1)
+    try:
+        for call in (c.bad_slots, lambda: gomel_amd.Cache(_Engine, 4), lambda: cache.from_cache(_Engine, c, [[1]])):
+            with pytest.raises(gomel_amd.GomelError) as err:
+                call()
+            assert err.value.status == 1
+    finally:
+        c._c = ctypes.c_void_p()

@@ -302,7 +302,8 @@ def _capture_child(rep):
         for call in (lambda: e.from_cache(c, [at], seeds=[3]), lambda: e.from_cache(c, [list(range(5, 25))], seeds=[3]),
                      lambda: e.from_cache(c, [list(range(5, 25))], seeds=[3], stream=named.cuda_stream),
                      lambda: b.upload_cache(c, at), lambda: b.upload_cache(c, np.arange(20)), lambda: b.upload_cache(c, at, stream=named),
-                     lambda: e.to_mel_cache([wave], c, list(range(n))), lambda: e.to_mel_cache([wave], c, list(range(n)), stream=named)):
+                     lambda: e.to_mel_cache([wave], c, list(range(n))), lambda: e.to_mel_cache([wave], c, list(range(n)), stream=named),
+                     c.bad_slots, lambda: e.cache(4)):
             with pytest.raises(gomel_amd.GomelError) as err:
                 call()
             assert err.value.status == 1
