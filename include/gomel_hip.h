@@ -283,7 +283,12 @@ int gomel_get_precision(const gomel_handle* h, int32_t iterations, int32_t* fp64
  *     lo   = min of the group's finite values, hi = max, each rounded to fp32 (beyond fp32: the largest fp32 number)
  *     step = fp32((hi - lo) / (2^bits - 1)), difference and quotient in fp64
  * and a value x is held as q = rint((x - lo) / step) -- evaluated in fp64, ties to even, clamped to 0 ... 2^bits - 1; 0 where step = 0 --
- * and reads as lo + q * step: at most half a step from x.  -inf is held as q = 0, +inf as the largest q; a group with no finite
+ * and reads as lo + q * step, which for |x| within fp32 is off by at most the sum of
+ *     step / 2
+ *     2^-24 of the larger of |lo| and |hi|, for fp64 frames (of the other types min and max are fp32 numbers)
+ *     2^-142, where step is below 2^-126 (a subnormal step is itself off by up to 2^-150)
+ *     the read's rounding: 2^-24 of the value (2^-53 for GOMEL_F64), then 2^-11 / 2^-8 of it for fp16 / bf16
+ * (a rounding at the end of a type's range may be one to infinity; a value beyond fp32 reads as one at the end of its group).  -inf is held as q = 0, +inf as the largest q; a group with no finite
  * value that is all -inf (all +inf) reads as that; a group that contains a NaN, or both infinities and nothing finite, reads as NaN.
  *   The cache has `n_slots` slots of one frame (gomel_cache_frame_bytes each, plus 4 bytes); slots never written read as zeros.
  * Pages, sequences and their tables are the caller's: a call takes `slots`, one int64 per frame (host or device memory), or NULL =

@@ -8,6 +8,7 @@ import types
 import numpy as np
 import pytest
 
+import cache_reference as ref
 from test_cache import _Engine, _cache
 
 
@@ -74,7 +75,6 @@ def _derivatives_child(rep):
     import torch
     import torch.autograd.forward_ad as fwd
     from gomel_amd import cache
-    import cache_reference as ref
 
     def kernel(fn, where, engine, x, p, seed, offset, out, stream):
         v = x.detach().numpy()
@@ -292,3 +292,41 @@ def test_calls_that_wait_are_refused_in_a_capture(monkeypatch):
             assert err.value.status == 1
     finally:
         c._c = ctypes.c_void_p()
+
+
+# ------------------------------------------------------------------------------------------------ how far a value reads from what was written
+def bound(x, lo, step, hi, dtype):
+    """include/gomel_hip.h's bound before the read's rounding, x [..] float64 values of one group each (lo, step, hi broadcast to them)."""
+    b = step.astype(np.float64) / 2 + np.where(step < 2.0 ** -126, 2.0 ** -142, 0.0)
+    if dtype == "float64":
+        b = b + 2.0 ** -24 * np.maximum(np.abs(lo.astype(np.float64)), np.abs(hi)) + 2.0 ** -150
+    return b * (1 + 2.0 ** -40)                          # the definition's own fp64 arithmetic
+
+
+def hard_groups(rng, n, K, dtype):
+    """Frames of every size and offset: spans from subnormal to the whole range, offsets far above the span, equal values."""
+    top = {"float64": 38, "float32": 38, "float16": 4, "bfloat16": 38}[dtype]
+    span = 10.0 ** rng.uniform(-44 if dtype != "float16" else -7, top, (n, 1, 1))
+    off = rng.choice([0.0, 1.0, 1e3, 1e-3], (n, 1, 1)) * span * rng.uniform(-2, 2, (n, 1, 1))
+    x = off + span * rng.random((n, K, 2)) * rng.choice([1.0, 1.0, 1e-6, 0.0], (n, 1, 1))
+    big = {"float64": 3.4e38, "float32": 3.4e38, "float16": 65504.0, "bfloat16": 3.38e38}[dtype]
+    return np.clip(x, -big, big)
+
+
+@pytest.mark.parametrize("dtype", ["float64", "float32", "float16", "bfloat16"])
+def test_the_contracts_bound(dtype):
+    rng = np.random.default_rng(12)
+    x = hard_groups(rng, 1500, 16, dtype)
+    x[:3] = [[1.0, 1.0 + 1e-9]], [[1000.0, 1000.001]], [[0.0, 370 * 2.0 ** -149]]
+    x = (ref.from_bf16(ref.to_bf16(x.astype(np.float32))) if dtype == "bfloat16" else x.astype(dtype)).astype(np.float64)
+    for bits in (8, 4):
+        for group in (0, 8):
+            q, lo, step = ref.quantise(x, bits, group)
+            of = np.arange(16) // (group or 16)
+            hi = x.reshape(len(x), -1, group or 16, 2).max((2, 3))
+            off = np.abs(ref.stands_for(x, bits, group) - x)
+            b = bound(x, lo[:, of, None], step[:, of, None], hi[:, of, None], dtype)
+            # stands_for's own sum: two roundings of 2^-53 of its larger operand
+            assert np.all(off <= b + 2.0 ** -52 * (np.abs(lo[:, of, None]) + 16 * np.abs(x))), (bits, group, np.max(off / np.maximum(b, 1e-300)))
+            if dtype in ("float64", "float32"):
+                assert np.any(off > step[:, of, None] * 0.51)         # half a step alone does not hold

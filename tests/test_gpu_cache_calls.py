@@ -7,7 +7,8 @@ import numpy as np
 import pytest
 
 import cache_reference as ref
-from test_gpu_cache import dev, engine, frames, held  # noqa: F401  (dev: the fixture)
+from test_cache_calls import bound, hard_groups
+from test_gpu_cache import TYPES, dev, engine, frames, held  # noqa: F401  (dev: the fixture)
 
 pytestmark = [pytest.mark.gpu]
 
@@ -525,3 +526,30 @@ def _bad_slots_child(rep):
 def test_no_bad_slot_is_lost_to_a_count_beside_a_running_call():
     import _children
     assert _children.run_child(_bad_slots_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ how far a value reads from what was written
+@pytest.mark.parametrize("dtype", TYPES)
+def test_reads_keep_the_contracts_bound(dev, dtype):  # noqa: F811
+    """Bound of include/gomel_hip.h with the read's rounding, for the type that was written and for float64."""
+    K, n = 16, 1500
+    e = engine(K)
+    x = held(hard_groups(np.random.default_rng(5), n, K, dtype), dtype)
+    for bits, group in ((8, 0), (4, 8)):
+        c = e.cache(n, bits, group)
+        c.write(dev.up(x, dtype))
+        _, lo, step = ref.quantise(x, bits, group)
+        of = np.arange(K) // (group or K)
+        hi = x.reshape(n, -1, group or K, 2).max((2, 3))
+        b = bound(x, lo[:, of, None], step[:, of, None], hi[:, of, None], dtype)
+        for out_type in {dtype, "float64"}:
+            out = dev.empty(x.size, out_type)
+            c.read(out)
+            got = dev.down(out, x.shape)
+            v = np.abs(x) + b
+            wide = 2.0 ** -53 if out_type == "float64" else 2.0 ** -24
+            room = v * wide * 1.001 + (v * ref.HALF[out_type] * 1.001 if out_type in ("float16", "bfloat16") else 0) + 2 * ref.TINY[out_type] + 2 * ref.TINY["float32"]
+            fits = v < {"float64": 1e300, "float32": 3.4e38, "float16": 65000.0, "bfloat16": 3.38e38}[out_type]
+            assert np.all(np.abs(got - x)[fits] <= (b + room)[fits]), (bits, group, out_type)
+        c.close()
+    e.close()
