@@ -553,3 +553,68 @@ def test_reads_keep_the_contracts_bound(dev, dtype):  # noqa: F811
             assert np.all(np.abs(got - x)[fits] <= (b + room)[fits]), (bits, group, out_type)
         c.close()
     e.close()
+
+
+# ------------------------------------------------------------------------------------------------ forms that other sizes do not reach
+@pytest.mark.parametrize("K,dtype", [(350, "float64"), (700, "float32"), (1400, "float16"), (1400, "bfloat16"), (161, "float64"), (383, "float64")])
+def test_rows_of_up_to_six_units_a_lane(dev, K, dtype):  # noqa: F811
+    """Rows of 321 ... 384 units of 16 bytes (six to each of 64 lanes), one scale a frame and groups, few frames and many; and their
+    neighbours of 3 and 6 units with a last one that is partial or missing."""
+    e = engine(K, Resolut=8192) if K > 700 else engine(K)
+    for bits, group in ((8, 0), (4, 0), (8, 16), (4, 64)):
+        for n in (5, 4500):                              # at most 4096: a wave for a frame
+            base = frames(8, K, K + n)
+            xd = held(base, dtype)
+            want, (q, lo, step) = ref.stands_for(xd, bits, group), ref.quantise(xd, bits, group)
+            of = np.arange(K) // (group or K)
+            size = np.abs(lo)[:, of, None] + q * step[:, of, None].astype(np.float64)
+            c = e.cache(n, bits, group)
+            which, slots = np.arange(n) % 8, np.random.default_rng(n).permutation(n).astype(np.int64)
+            src, val, out, at = dev.up(base[which], dtype), dev.empty(n * 2 * K, dtype), dev.empty(n * 2 * K, dtype), dev.up(slots, "int64")
+            c.write(src, slots=at, values=val)
+            c.read(out, slots=at)
+            got, back = dev.down(out, (n, K, 2)), dev.down(val, (n, K, 2))
+            assert np.array_equal(got, back), (bits, group, n)
+            for i in range(min(n, 8)):
+                assert ref.close(got[i], (want[i], size[i]), dtype, 1), (bits, group, n, i)
+                assert np.array_equal(got[which == i], np.broadcast_to(got[i], got[which == i].shape)), (bits, group, n, i)
+            c.close()
+    e.close()
+
+
+def _large_read_with_dropout_child(rep):
+    """Outputs of 64 MB and more with dropout: bit for bit what small reads give, each at the counter of its first element."""
+    import torch
+    torch.zeros(1, device="cuda")
+    K = 192
+    e = engine(K, Device=0)
+    for dtype in (torch.float16, torch.bfloat16, torch.float32, torch.float64):
+        n = (64 << 20) // (2 * K * torch.empty(0, dtype=dtype).element_size()) + 1003
+        for bits, group in ((8, 0), (4, 32)):
+            c = e.cache(n, bits, group)
+            at = torch.randperm(n, device="cuda")
+            c.write((torch.randn(n, K, 2, device="cuda") * 3).to(dtype))
+            large, plain = torch.empty(n, K, 2, device="cuda", dtype=dtype), torch.empty(n, K, 2, device="cuda", dtype=torch.float64 if dtype == torch.float64 else torch.float32)
+            for p, seed, offset in ((0.25, 3, 0), (0.6, 2 ** 63 + 1, 7)):
+                c.read(large, slots=at, p=p, seed=seed, offset=offset)
+                small = torch.empty_like(large)
+                step = 9000
+                for r in range(0, n, step):
+                    c.read(small[r:r + step], slots=at[r:r + step], p=p, seed=seed, offset=offset + 2 * K * r)
+                assert torch.equal(large, small), (dtype, bits, group, p)
+                # against the definition: dropout of the wide read, rounded once
+                c.read(plain, slots=at)
+                for r in (0, n // 2, n - 40):
+                    drop = ref.dropped(p, seed, offset + 2 * K * r, 40 * 2 * K).reshape(40, K, 2)
+                    want = np.where(drop, 0.0, plain[r:r + 40].double().cpu().numpy() / (1 - p))
+                    assert ref.close(large[r:r + 40].double().cpu().numpy(), want, str(dtype).replace("torch.", ""), 2), (dtype, bits, group, p, r)
+            c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_large_reads_with_dropout_in_every_type():
+    import _children
+    assert _children.run_child(_large_read_with_dropout_child)["ok"]
