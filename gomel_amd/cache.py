@@ -98,10 +98,18 @@ def _as_stream(stream, device):
 
 
 def _used_on(stream, *arrays):
-    """Tells torch's allocator that a call on a named stream still uses these tensors: their memory is not handed on before it is through."""
-    for a in arrays:
-        if _Tensor is not None and isinstance(a, _Tensor):
-            a.record_stream(_as_stream(stream, a.device))
+    """Keeps the memory of these tensors, should they be dropped now, from being handed on before a call on a named stream is through with
+    it.  On a stream of torch's its allocator is told.  It would ask a foreign one (an integer handle) when the tensors are freed, which
+    may be after the stream's end: there torch's current stream waits for the call."""
+    tensors = [a for a in arrays if isinstance(a, _Tensor)] if _Tensor is not None else ()
+    if not tensors:
+        return
+    cuda, device = _torch.cuda, tensors[0].get_device()
+    if isinstance(stream, cuda.Stream) and not isinstance(stream, cuda.ExternalStream):
+        for a in tensors:
+            a.record_stream(stream)
+    elif int(getattr(stream, "cuda_stream", stream)) != _raw_stream(device) and not _capturing(None, device) and not _capturing(stream, device):
+        cuda.current_stream(device).wait_stream(_as_stream(stream, device))
 
 
 def _device_of(engine_device, *devices):

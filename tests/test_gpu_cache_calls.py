@@ -618,3 +618,46 @@ def _large_read_with_dropout_child(rep):
 def test_large_reads_with_dropout_in_every_type():
     import _children
     assert _children.run_child(_large_read_with_dropout_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ streams that are not torch's
+def _foreign_stream_child(rep):
+    """A call on a stream that the program makes and ends by itself, before the tensors go."""
+    import torch
+    import gomel_amd
+    torch.zeros(1, device="cuda")
+    hip = ctypes.CDLL(gomel_amd.hip_runtime_path())
+    hip.hipStreamCreateWithFlags.argtypes = [ctypes.POINTER(ctypes.c_void_p), ctypes.c_uint]
+    hip.hipStreamSynchronize.argtypes = hip.hipStreamDestroy.argtypes = [ctypes.c_void_p]
+    e = engine(80, Device=0)
+    c = e.cache(500)
+    x, at = torch.randn(500, 80, 2, device="cuda"), torch.randperm(500, device="cuda")
+    want, y_want = torch.empty_like(x), torch.empty_like(x)
+    c.write(x, slots=at, values=want)
+    e.dropout(x, 0.5, 1, out=y_want)
+    for kind in (int, lambda h: torch.cuda.ExternalStream(h)):
+        s = ctypes.c_void_p()
+        assert hip.hipStreamCreateWithFlags(ctypes.byref(s), 1) == 0
+        out, val, y, at2 = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x), at.clone()
+        torch.cuda.synchronize()
+        named = kind(s.value)
+        c.write(x, slots=at2, values=val, stream=named)
+        c.read(out, slots=at2, stream=named)
+        e.dropout(x, 0.5, 1, out=y, stream=named)
+        del at2
+        torch.full_like(at, 3)                           # torch's stream is behind the calls: no wait is needed to reuse or to read
+        assert torch.equal(out, want) and torch.equal(val, want) and torch.equal(y, y_want)
+        assert hip.hipStreamSynchronize(s) == 0 and hip.hipStreamDestroy(s) == 0
+        del out, val, y, named                           # freed after the stream's end
+        torch.cuda.synchronize()
+        assert torch.empty_like(x).fill_(1).sum() == x.numel()
+    c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_calls_on_a_stream_that_ends_before_its_tensors():
+    import _children
+    assert _children.run_child(_foreign_stream_child)["ok"]
