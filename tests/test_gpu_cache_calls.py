@@ -661,3 +661,101 @@ def _foreign_stream_child(rep):
 def test_calls_on_a_stream_that_ends_before_its_tensors():
     import _children
     assert _children.run_child(_foreign_stream_child)["ok"]
+
+
+def _named_in_a_capture_child(rep):
+    """Streams named inside a capture: the capturing one, as an object and as a handle, and one forked from it."""
+    import torch
+    torch.zeros(1, device="cuda")
+    n, K = 300, 80
+    e = engine(K, Device=0)
+    c = e.cache(n)
+    x, at = torch.randn(n, K, 2, device="cuda"), torch.randperm(n, device="cuda")
+    val, out, out2, y = (torch.zeros_like(x) for _ in range(4))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        cur = torch.cuda.current_stream()
+        c.write(x, slots=at, values=val, stream=cur)
+        c.read(out, slots=at, stream=cur.cuda_stream)
+        side.wait_stream(cur)
+        c.read(out2, slots=at.clone(), stream=side)
+        e.dropout(x, 0.5, 3, out=y, stream=side.cuda_stream)
+        cur.wait_stream(side)
+    for i in range(4):
+        x.copy_(torch.randn_like(x))
+        g.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (val, out, out2, y)]
+        c.write(x, slots=at, values=val)                 # the program's own eager work
+        e.dropout(x, 0.5, 3, out=y)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, val) for a in got[:3]) and torch.equal(got[3], y), i
+    c.close()
+    e.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_streams_named_inside_a_capture():
+    import _children
+    assert _children.run_child(_named_in_a_capture_child)["ok"]
+
+
+# ------------------------------------------------------------------------------------------------ host memory in several pieces
+def test_host_frames_of_several_staging_pieces(dev):  # noqa: F811
+    """90 MB of host frames go through 32 MB of staging: bit for bit the device path, by slots (one named again in a later piece, padding) and
+    in order, dense and apart, with dropout's counter running on."""
+    K, n = 192, 30000
+    e = engine(K)
+    x = frames(n, K, 4)
+    rng = np.random.default_rng(2)
+    slots = rng.permutation(n + 100)[:n].astype(np.int64)
+    slots[100], slots[n - 50] = slots[n - 7], slots[40]  # first and third piece
+    slots[[5, 15000, n - 1]] = -1
+    src, at = dev.up(x, "float64"), dev.up(slots, "int64")
+    val, out, drop = (dev.up(np.full(x.shape, 9.0), "float64") for _ in range(3))
+    c, h = e.cache(n + 100, 8, 16), e.cache(n + 100, 8, 16)
+    c.write(src, slots=at, values=val)
+    c.read(out, slots=at)
+    c.read(drop, slots=at, p=0.3, seed=8, offset=1)
+    want, want_val, want_drop = (dev.down(d, x.shape) for d in (out, val, drop))
+    wide = np.full((n, K + 3, 2), 9.0)
+    wide[:, 1:K + 1] = x
+    values = np.full_like(x, 9.0)
+    h.write(wide[:, 1:K + 1], slots=slots, values=values)
+    assert np.array_equal(values, want_val)
+    assert np.array_equal(h.read(np.full_like(x, 9.0), slots=slots), want)
+    assert np.array_equal(h.read(np.full_like(x, 9.0), slots=slots, p=0.3, seed=8, offset=1), want_drop)
+    wide[:] = 9.0
+    h.read(wide[:, 1:K + 1], slots=at)                   # slots on the device
+    assert np.array_equal(wide[:, 1:K + 1], want) and np.all(wide[:, 0] == 9) and np.all(wide[:, K + 1:] == 9)
+    h.write(x, first=70)                                 # in order
+    c.write(src, first=70)
+    c.read(out, first=70)
+    assert np.array_equal(h.read(np.empty_like(x), first=70), dev.down(out, x.shape))
+    h.write(wide[:, 1:K + 1], slots=slots, values=wide[:, 1:K + 1])            # in place
+    assert np.all(wide[:, 0] == 9) and np.all(wide[:, K + 1:] == 9) and np.all(wide[5, 1:K + 1] == 9)
+    for k in (c, h):
+        k.close()
+    e.close()
+
+
+@pytest.mark.parametrize("rows,cols,apart", [(9, 1_500_001, 3), (3, 5_000_003, 0), (2, 5_000_003, 4), (1, 9_000_001, 0)])
+def test_host_dropout_of_several_staging_pieces(dev, rows, cols, apart):  # noqa: F811
+    """Pieces of whole rows, and of one row where a row alone is more than the staging buffer."""
+    e = engine(80)
+    rng = np.random.default_rng(rows)
+    wide = rng.normal(size=(rows, cols + apart))
+    x = wide[:, apart:]
+    src, out = dev.up(x, "float64"), dev.empty(x.size, "float64")
+    e.dropout(src, 0.4, 77, 5, out=out)
+    want = dev.down(out, x.shape)
+    assert np.array_equal(want == 0, ref.dropped(0.4, 77, 5, x.size).reshape(x.shape))
+    assert np.array_equal(e.dropout(x, 0.4, 77, 5), want)
+    keep = wide[:, :apart].copy()
+    e.dropout_backward(x, 0.4, 77, 5, out=x)
+    assert np.array_equal(x, want) and np.array_equal(wide[:, :apart], keep)
+    e.close()
