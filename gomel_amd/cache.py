@@ -1,8 +1,8 @@
 """The spectrogram cache and dropout over the C ABI (gomel_cache_*, gomel_dropout* in include/gomel_hip.h: formulas and contract there).
 
 What the calls take: numpy arrays (float64, float32, float16; copied through a staging buffer, the call returns when it is done), torch
-tensors on the engine's device (those types and bfloat16; the call queues kernels on torch's current stream, or on `stream`) and
-`DevicePointer`s.  There is no CPU fallback."""
+tensors on the engine's device (those types and bfloat16; the call only queues kernels) and `DevicePointer`s.  A call runs on `stream`,
+else on torch's current stream where torch is in use, else on the default stream.  There is no CPU fallback."""
 import ctypes
 import sys
 from operator import index as _index     # any integer's value: Python's, numpy's, a torch scalar's

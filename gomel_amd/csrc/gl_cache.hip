@@ -56,7 +56,7 @@ GL_DEV float code_of(double v, Scale s, float levels) {
 //   fp32 (and the 16-bit types): v - lo is off by 2^-24 of itself, v_rcp_f32 by 2^-23, the product by 2^-24: 2^-22 of a quotient of at
 // most `levels` (and a little), so levels * 2^-21 is twice what is needed; one value in 4000 is that near at 8 bits.  Instructions of
 // either width cost the same here, but the definition takes twice as many: a write of 16-bit frames was bound by them (192 bands: 740
-// vector instructions per wave and 193 us for 409 600 frames with values, now 400 and 158).
+// vector instructions per wave and 193 us for 409 600 frames with values, now 489 and 159).
 //   fp64: 2^-51 of the quotient; 2^-33 is far beyond it and as rare as never.
 // Whatever is not a number in between (an infinite value, a step whose reciprocal fp32 does not hold) fails the comparison and goes there too.
 template <int N> GL_DEV void quantise(const float* v, Scale s, float per, float levels, float* q) {
@@ -363,8 +363,9 @@ template <class T, int S> GL_DEV void put_unit(const WriteArgs& a, uint8_t* row,
 // A frame -- or, of a wide grouped one, a segment of it -- lies in the registers of its lanes (Spread).  Its extremes are joined across
 // those lanes (a group's across the lanes of the group), the codes follow from the same registers: the frames are read once.  Bound by
 // HBM in fp32 and fp64: 102 400 x 192 bands of fp32 to 8 bits with values 56 us (6.3 TB/s) into slots in order, 60 with the claims
-// of slots in any order; 409 600 of fp64 to 4 bits 440 us (5.95 TB/s).  In 16-bit types the vector unit is busy for two thirds of the time
-// (409 600 of bf16 to 8 bits 139 and 158 us).
+// of slots in any order; 409 600 of fp64 to 4 bits 440 us (5.95 TB/s).  16-bit types are bound by the vector unit as
+// well: 409 600 of bf16 to 8 bits 109 us without values (77 for the bytes; 421 instructions a wave, 70 us of issue) and 159 with (128; 489),
+// in groups of 64 bands 119 (602, 100 us: each unit's lanes work their group's scale out) and 159 (669), of 16 bands 126 and 171.
 template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256) void k_write(WriteArgs a) {
     typedef typename Wide<T>::type W;
     const int lanes = 1 << a.p.lanes_log2, l = (int)threadIdx.x & (lanes - 1);
@@ -443,7 +444,7 @@ template <class T, int NC, bool GROUPED, int S> __global__ __launch_bounds__(256
 }
 
 // A frame under one scale that is too wide for a wave's registers: a block per frame, which reads it twice (the second time out of the
-// caches: at most 256 KB).
+// caches: at most 256 KB).  4 000 x 2 600 bands of fp32 to 8 bits 32 us (17 for the bytes), 40 000 with values 415 (302).
 template <class T> __global__ __launch_bounds__(256) void k_write_wide(WriteArgs a) {
     typedef typename Wide<T>::type W;
     __shared__ W s_mn[4], s_mx[4];
@@ -581,7 +582,8 @@ template <class T, int BITS, int NC, bool S> __global__ __launch_bounds__(256) v
     }
 }
 // The same with dropout: bound by the generator as dropout in 16 bits is (54 912 x 80 bands to bf16: 8.8 us, of which 5.6 are its products),
-// so the lane's units go through one loop body; loading the next unit's codes ahead changed nothing.
+// so the lane's units go through one loop body; loading the next unit's codes ahead changed nothing.  102 400 x 192 bands: bf16 23.5 us,
+// fp32 30.4 (6.5 TB/s) and fp64 49.4 (7.2, codes partly from the caches): there HBM is the bound.
 template <class T, int BITS, bool S> __global__ __launch_bounds__(256) void k_read_drop(ReadArgs a) {
     typedef typename Wide<T>::type W;
     int64_t r;
@@ -633,7 +635,8 @@ template <class T, bool S, bool LN> __global__ __launch_bounds__(256) void k_dro
     for (int j = 0; j < UV<T>; j++) x.v[j] = drop_or<T>(widen(x.v[j]), a.drop, u[j]);
     x.template store<S>((T*)a.y + e0 + t, n);
 }
-// Rows apart, each with units of its own (Walk).
+// Rows apart, each with units of its own (Walk).  102 400 rows of 384 elements 390 apart: bf16 25.9 us, fp32 55.2 (6.1 and 5.7 TB/s); of 322,
+// 384 apart: 34.8 and 49.7 (3.8 and 5.3): a 41st unit of two elements to every row.
 template <class T, bool S> __global__ __launch_bounds__(512) void k_dropout_rows(DropArgs a) {
     int64_t r, k;
     if (!walk_unit(a.w, a.block0 + blockIdx.x, &r, &k)) return;
@@ -740,7 +743,8 @@ hipError_t dropout_device(int type, const void* x, size_t xs, void* y, size_t ys
 
 constexpr size_t kStageBytes = (size_t)32 << 20;
 // Frames of a write up to which each looks through the later slots itself, per lane that looks; more claim theirs first.  The search grows
-// with the square (192 bands of bf16, 16 lanes: 6.4 us for 256 frames, 8.0 for 1024, 10.2 for 2048), the claims cost a launch (8.8 ... 9.1).
+// with the square, the claims cost a launch (192 bands of bf16, slots in any order: 64 lanes look, 6.0 us for 1 024 and for 2 048 frames, 8.9
+// for 4 096; by claims 8 192 frames 9.1; in slot order, with neither, 5.6 ... 6.5.  16 lanes took 10.2 for 2 048).
 constexpr size_t kScanPerLane = 64;
 
 // Rows between host memory (stride elements apart) and a dense device buffer

@@ -29,6 +29,8 @@
 extern "C" {
 #endif
 
+/* Counted up when something that is here changes.  Entry points may be added under the same number: the number says that what a host was
+ * built against still means the same, not that a library has every later entry point (one that lacks it does not link, or resolve). */
 #define GOMEL_HIP_ABI_VERSION 6
 
 typedef enum gomel_status {
