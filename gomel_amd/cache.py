@@ -36,11 +36,12 @@ class _AnyLevel:
 def _version_counter(torch):
     """torch.autograd.graph.increment_version without its wrapper (0.2 us), where that does the same."""
     try:
-        probe = torch.empty(0)
-        torch._C._increment_version((probe,))
-        if probe._version == 1:
-            return torch._C._increment_version
-    except (AttributeError, TypeError):
+        with torch.inference_mode(False):        # (its tensors have no version)
+            probe = torch.empty(0, device="cpu")
+            torch._C._increment_version((probe,))
+            if probe._version == 1:
+                return torch._C._increment_version
+    except (AttributeError, TypeError, RuntimeError):
         pass
     return torch.autograd.graph.increment_version
 

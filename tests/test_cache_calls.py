@@ -330,3 +330,23 @@ def test_the_contracts_bound(dtype):
             assert np.all(off <= b + 2.0 ** -52 * (np.abs(lo[:, of, None]) + 16 * np.abs(x))), (bits, group, np.max(off / np.maximum(b, 1e-300)))
             if dtype in ("float64", "float32"):
                 assert np.any(off > step[:, of, None] * 0.51)         # half a step alone does not hold
+
+
+# ------------------------------------------------------------------------------------------------ the first tensor of a process
+def _first_tensor_child(rep):
+    import torch
+    from gomel_amd import cache
+    with torch.inference_mode():
+        t = torch.zeros(3, 4, 2)
+        assert cache._is_tensor(t)
+        cache._written(t)                                # has no version to count
+    u = torch.zeros(3)
+    cache._written(u)
+    assert u._version == 1
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+def test_the_first_tensor_may_be_an_inference_tensor():
+    import _children
+    assert _children.run_child(_first_tensor_child)["ok"]
