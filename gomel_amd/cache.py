@@ -337,8 +337,9 @@ class Cache:
         """Gives the memory back -- in a capture (gomel_cache_destroy waits for the device, which would end it) when the next call of any
         cache is made outside one."""
         if self._c:
+            later = _capturing(None, self.device)
             c, self._c = self._c, ctypes.c_void_p()
-            if _capturing(None, self.device):
+            if later:
                 _left.append((c, self.device))
             else:
                 _destroy_left(self.device)

@@ -290,8 +290,9 @@ int gomel_get_precision(const gomel_handle* h, int32_t iterations, int32_t* fp64
  *     2^-24 of the larger of |lo| and |hi|, for fp64 frames (of the other types min and max are fp32 numbers)
  *     2^-142, where step is below 2^-126 (a subnormal step is itself off by up to 2^-150)
  *     the read's rounding: 2^-24 of the value (2^-53 for GOMEL_F64), then 2^-11 / 2^-8 of it for fp16 / bf16
- * (a rounding at the end of a type's range may be one to infinity; a value beyond fp32 reads as one at the end of its group).  -inf is held as q = 0, +inf as the largest q; a group with no finite
- * value that is all -inf (all +inf) reads as that; a group that contains a NaN, or both infinities and nothing finite, reads as NaN.
+ * (a rounding at the end of a type's range may be one to infinity; a value beyond fp32 reads as one at the end of its group).  -inf is held
+ * as q = 0, +inf as the largest q; a group with no finite value that is all -inf (all +inf) reads as that; a group that contains a NaN, or
+ * both infinities and nothing finite, reads as NaN.
  *   The cache has `n_slots` slots of one frame (gomel_cache_frame_bytes each, plus 4 bytes); slots never written read as zeros.
  * Pages, sequences and their tables are the caller's: a call takes `slots`, one int64 per frame (host or device memory), or NULL =
  * the slots first, first + 1, ...  A negative slot marks padding: nothing is written to the cache, and the frame's row of the output
@@ -304,7 +305,8 @@ int gomel_get_precision(const gomel_handle* h, int32_t iterations, int32_t* fp64
  * buffer and returns when it is done (not while `stream` is being captured: GOMEL_ERR_BAD_CONFIG).  Calls that touch the same
  * slots on different streams are the caller's to order.  `n` = 0 is a call without work.
  *   gomel_cache_write: quantises n frames.  values != NULL also receives what the cache now stands for, rounded to `type` (what a
- * generating model is to be conditioned on; a straight-through gradient of it is the identity); values may be frames itself (same stride) but must not overlap it otherwise.
+ * generating model is to be conditioned on; a straight-through gradient of it is the identity); values may be frames itself (same stride)
+ * but must not overlap it otherwise.
  *   gomel_cache_read: dequantises n frames (fp32 arithmetic; fp64 for GOMEL_F64), rounded once to `type`.  p > 0 applies dropout
  * (below) to the values read, element index = position in the dense [n][2 * NumMels] output.
  * The cache keeps nothing of the handle (its NumMels and device are copied): either may be destroyed first.  gomel_cache_create
