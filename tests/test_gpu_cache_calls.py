@@ -761,3 +761,45 @@ def test_host_dropout_of_several_staging_pieces(dev, rows, cols, apart):  # noqa
     e.dropout_backward(x, 0.4, 77, 5, out=x)
     assert np.array_equal(x, want) and np.array_equal(wide[:, :apart], keep)
     e.close()
+
+
+def test_every_call_survives_a_launch_that_fails(dev):  # noqa: F811
+    """Device and host memory, the second of several pieces, FromMel's upload and ToMel's write: status 8 each, and the next call works."""
+    import gomel_amd
+    from gomel_amd import _lib
+    fail = _lib.lib().gomel_debug_fail_launch
+    fail.restype, fail.argtypes = None, [ctypes.c_int]
+    K, n = 192, 30000
+    e = engine(K, GriffinLimIterations=2)
+    c = e.cache(n)
+    x = frames(n, K, 3)
+    src, out = dev.up(x, "float64"), dev.empty(x.size, "float64")
+    host, small, y = np.empty_like(x), np.empty((5, K, 2)), np.zeros(9_000_001)
+    wave = np.random.default_rng(0).normal(size=30000)
+    m = len(e.to_mel_batch([wave])[0]) // K
+    b = gomel_amd.Batch(e, [40 * K])
+    calls = {"write": (1, lambda: c.write(src)), "read": (1, lambda: c.read(out)), "read, dropout": (1, lambda: c.read(out, p=0.5)),
+             "host write": (1, lambda: c.write(x[:5])), "second piece": (2, lambda: c.write(x)), "host read": (1, lambda: c.read(small)),
+             "third piece": (3, lambda: c.read(host)), "dropout": (1, lambda: e.dropout(src, 0.5, 1, out=out)), "host dropout": (1, lambda: e.dropout(small, 0.5, 1)),
+             "second piece of dropout": (2, lambda: e.dropout(y, 0.5, 1)), "backward": (1, lambda: e.dropout_backward(src, 0.5, 1, out=out)),
+             "upload_cache": (1, lambda: b.upload_cache(c, np.arange(40))), "from_cache": (1, lambda: e.from_cache(c, [np.arange(40)])),
+             "to_mel_cache": (1, lambda: e.to_mel_cache([wave], c, np.arange(m)))}
+    for name, (nth, call) in calls.items():
+        call()
+        fail(nth)
+        try:
+            with pytest.raises(gomel_amd.GomelError) as err:
+                call()
+            assert err.value.status == 8, name
+        finally:
+            fail(0)
+        if name == "upload_cache":
+            with pytest.raises(gomel_amd.GomelError):
+                b.run()                                  # not uploaded any more
+        call()
+    c.write(src)
+    c.read(out)
+    assert np.array_equal(c.read(host), dev.down(out, x.shape))
+    b.close()
+    c.close()
+    e.close()
