@@ -105,12 +105,14 @@ hipStream_t handle_stream(const gomel_handle* h) { return h->stream; }
 hipError_t handle_stage(gomel_handle* h, size_t bytes, void** p) { std::lock_guard<std::mutex> lk(h->mu); return (hipError_t)h->pool.alloc(p, bytes); }
 void handle_unstage(gomel_handle* h, void* p) { std::lock_guard<std::mutex> lk(h->mu); h->pool.release(p); }
 
-// Queues `s` behind what is queued on the caller's stream.
+// Queues `s` behind what is queued on the caller's stream and, where that is not through yet, waits for it: a call that then enters the
+// device gate would otherwise keep persistent launches out for as long as the caller's work takes.
 static hipError_t follow(hipStream_t s, hipStream_t caller) {
     hipEvent_t ev = nullptr;
     hipError_t e = hipEventCreateWithFlags(&ev, hipEventDisableTiming);
     if (e == hipSuccess) e = hipEventRecord(ev, caller);
     if (e == hipSuccess) e = hipStreamWaitEvent(s, ev, 0);
+    if (e == hipSuccess && hipEventQuery(ev) != hipSuccess) { (void)hipGetLastError(); e = hipEventSynchronize(ev); }
     if (ev) (void)hipEventDestroy(ev);
     return e;
 }
@@ -1961,6 +1963,7 @@ static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* con
     if (slots_kind < 0) return GOMEL_ERR_BAD_CONFIG;
     if (!slots_kind)
         for (size_t f = 0; f < tot_f; f++) if (into->slots[f] >= 0 && (uint64_t)into->slots[f] >= into->c->n_slots) return GOMEL_ERR_TABLE_RANGE;
+    if (into) HIPCHK(follow(h->stream, into->caller));
     GateOrdinary gate_o; gate_o.enter(h, h->stream);   // synchronous entry point: the gate is left (destructor) after its streams have drained
     double *d_wave = nullptr, *d_smag = nullptr, *d_out = nullptr;
     v2d *d_bigA = nullptr, *d_bigB = nullptr;   // frame lengths above 8192: the convolution's scratch (gl_big.hpp)
@@ -1985,7 +1988,6 @@ static int to_mel_batch_guarded(gomel_handle* h, size_t n_utt, const double* con
         else if (hipMemcpyAsync(d_slots, slots, tot_f * 8, hipMemcpyHostToDevice, h->stream) != hipSuccess) rc = GOMEL_ERR_HIP;
         slots = d_slots;
     }
-    if (!rc && into && follow(h->stream, into->caller) != hipSuccess) rc = GOMEL_ERR_HIP;
     // Chunks of ~32 MB of samples, pipelined over the handle's three streams as in FromMel's batch call: chunk c+1's waveforms go up
     // while chunk c is transformed and chunk c-1's log-mel comes down (a 256 x 10 s call is H2D-bound: 0.9 GB up, 0.27 GB down,
     // 1.5 ms of kernels -- 28.7 ms one thing after the other, the upload's 18 ms plus a chunk's worth overlapped).  The device

@@ -803,3 +803,52 @@ def test_every_call_survives_a_launch_that_fails(dev):  # noqa: F811
     b.close()
     c.close()
     e.close()
+
+
+def _gate_child(rep):
+    """Calls that wait for the caller's stream wait outside the gate: a persistent launch of another engine is let in meanwhile."""
+    import threading
+    import time
+    import torch
+    import gomel_amd
+    torch.zeros(1, device="cuda")
+    K = 80
+    one = engine(K, Device=0, Resolut=1024, Window=256, MelFmax=8000, GriffinLimIterations=50)
+    one.set_path(3)                                      # persistent
+    one.set_precision(32)
+    run = gomel_amd.Batch(one, [4 * K])
+    run.upload([frames(4, K, 3).reshape(-1, 2)], None, [1])
+    other = engine(K, Device=0)
+    c = other.cache(64)
+    c.write(frames(64, K, 1))
+    b = gomel_amd.Batch(other, [40 * K])
+    wave = np.random.default_rng(0).normal(size=30000)
+    n = len(other.to_mel_batch([wave])[0]) // K
+    side = torch.cuda.Stream()
+    assert run.run_timed()["fast_path"] == 2
+    for what in (lambda: b.upload_cache(c, np.arange(40), stream=side), lambda: other.to_mel_cache([wave], c, np.arange(n), stream=side)):
+        what()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):                    # busy for a while, and the GPU is not
+            for _ in range(20):
+                torch.cuda._sleep(10_000_000)
+        waiting = threading.Thread(target=what)
+        t0 = time.perf_counter()
+        waiting.start()
+        time.sleep(0.005)
+        paths = []
+        while waiting.is_alive() and not side.query() and time.perf_counter() - t0 < 5:
+            paths.append(run.run_timed()["fast_path"])
+        waiting.join()
+        assert len(paths) > 1 and 2 in paths, paths
+        torch.cuda.synchronize()
+    for k in (b, run, c, one, other):
+        k.close()
+    rep.result({"ok": True})
+
+
+@pytest.mark.torch_child
+@pytest.mark.guard(700)
+def test_waiting_for_the_callers_stream_keeps_no_persistent_launch_out():
+    import _children
+    assert _children.run_child(_gate_child)["ok"]
